@@ -3,7 +3,8 @@
 Public API (the names of the reference package ``wbridge``, ``wbridge/__init__.py:3-17``):
 ``WeightSender``, ``WeightReceiver``, ``WeightReceiverController``, ``WeightData``,
 ``dtype_str_to_torch``, ``dtype_to_str``; plus ``TransferConfig`` and the layout adapters
-``MegatronLayout`` / ``FSDPLayout`` (trainers) and ``SGLangLayout`` (rollout).
+``MegatronLayout`` / ``FSDPLayout`` (trainers) and ``SGLangLayout`` (rollout), and the operators
+of an RL step beside the sync: ``token_logprobs``, ``AdamW`` and ``grad_norm``.
 """
 from .core.shard import (WeightData, check_shard_compatibility, original_total_numel,
                          shards_iterator)
@@ -25,6 +26,12 @@ def __getattr__(name):
     if name in ("SGLangLayout", "VLLMLayout"):
         from .parallel import sglang
         return getattr(sglang, name)
+    if name in ("token_logprobs", "TokenLogprobs"):
+        from .ops import logprobs
+        return getattr(logprobs, name)
+    if name in ("AdamW", "grad_norm"):
+        from .ops import optim
+        return getattr(optim, name)
     raise AttributeError(name)
 
 
@@ -32,5 +39,6 @@ __all__ = [
     "WeightData", "WeightSender", "WeightReceiver", "WeightReceiverController", "TransferConfig",
     "check_shard_compatibility", "shards_iterator", "original_total_numel", "dtype_str_to_torch",
     "dtype_to_str", "MegatronLayout", "FSDPLayout", "HFLayout", "SGLangLayout", "VLLMLayout",
+    "token_logprobs", "TokenLogprobs", "AdamW", "grad_norm",
 ]
 __version__ = "0.1.0"

@@ -14,6 +14,7 @@
 #include "wb_common.h"
 #include "wb_cpu.h"
 #include "wb_ipc.h"
+#include "wb_learn.h"
 #include "wb_splitq.h"
 #include "wb_synth.h"
 #include "wb_transfer.h"
@@ -276,6 +277,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mc_map", [](uint64_t mc, size_t size, int dev) { return vmm_tuple(wb::mc_map(mc, size, dev)); });
   m.def("mem_release", &wb::mem_release);
   m.def("va_unmap", &wb::va_unmap);
+  wb::bind_learn(m);
   m.attr("ITEM_SIZE") = (int)sizeof(wb::Item);
   m.attr("QDESC_SIZE") = (int)sizeof(wb::QuantDesc);
   m.attr("QWORK_SIZE") = (int)sizeof(wb::QuantWork);

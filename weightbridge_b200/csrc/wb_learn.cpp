@@ -1,0 +1,531 @@
+// Python bindings of the operators beside the sync: token log probabilities (wb_logprobs.cu) and
+// the optimizer kernels (wb_optim.cu).  Argument checks live here: everything a kernel relies on
+// (types, sizes, strides, devices) is checked on the host before a launch, and a call that does not
+// fit raises ValueError.  Outputs and scratch come from torch's allocator on the current stream of
+// the tensors' device, and the kernels run on that stream, so calls on different streams share nothing.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime.h>
+#include <torch/extension.h>
+
+#include <array>
+#include <cmath>
+#include <limits>
+#include <optional>
+#include <stdexcept>
+#include <string>
+#include <vector>
+
+#include "wb_learn.h"
+#include "wb_logprobs.h"
+#include "wb_optim.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using at::Tensor;
+
+[[noreturn]] void bad(const std::string& what) { throw std::invalid_argument(what); }
+
+void check(cudaError_t e, const char* what) {
+  if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+uint32_t float_code(at::ScalarType t) {
+  switch (t) {
+    case at::kBFloat16: return wb::DT_BF16;
+    case at::kHalf: return wb::DT_F16;
+    case at::kFloat: return wb::DT_F32;
+    default: return 0;
+  }
+}
+
+std::string shape_of(const Tensor& t) {
+  std::string s = "[";
+  for (int64_t d = 0; d < t.dim(); ++d) s += (d ? ", " : "") + std::to_string(t.size(d));
+  return s + "]";
+}
+
+int sm_count(int device) {
+  static std::array<int, 64> known{};          // one attribute query per device; the value never changes
+  int v = device < 64 ? known[device] : 0;
+  if (!v) {
+    check(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device), "cudaDeviceGetAttribute");
+    if (device < 64) known[device] = v;
+  }
+  return v;
+}
+
+// -- token log probabilities ----------------------------------------------------------------------
+// The leading dimensions as (outer, inner) with one stride each: any tensor of up to two leading
+// dimensions, and more where they merge.
+struct Lead { int64_t outer = 1, inner = 1, s_outer = 0, s_inner = 0; };
+
+std::optional<Lead> lead_of(const Tensor& t, int64_t dims) {
+  std::vector<std::pair<int64_t, int64_t>> d;      // (size, stride), merged
+  for (int64_t k = 0; k < dims; ++k) {
+    const int64_t n = t.size(k), s = t.stride(k);
+    if (n == 1) continue;
+    if (!d.empty() && d.back().second == n * s) d.back() = {d.back().first * n, s};
+    else d.push_back({n, s});
+  }
+  if (d.size() > 2) return std::nullopt;
+  Lead l;
+  if (d.size() == 2) l.outer = d[0].first, l.s_outer = d[0].second;
+  if (!d.empty()) l.inner = d.back().first, l.s_inner = d.back().second;
+  return l;
+}
+
+struct LogprobOptions {
+  int64_t vocab = 0, ignore_index = -100;
+  double temperature = 1.0;
+  int64_t top_k = 0;
+};
+
+wb::LogprobRows rows_of(const Tensor& logits, const Tensor& tokens, const LogprobOptions& o, Tensor& tokens_kept) {
+  const int64_t lead = logits.dim() - 1;
+  auto l = lead_of(logits, lead);
+  if (!l) bad("token_logprobs: logits of shape " + shape_of(logits) + " have more than two leading dimensions that do not "
+              "merge into one; pass a tensor of two leading dimensions");
+  wb::LogprobRows in{};
+  // the tokens follow the logits' split of the rows; where their own strides do not, a packed copy does
+  tokens_kept = tokens;
+  auto t = lead_of(tokens, lead);
+  if (!t || t->inner != l->inner || t->outer != l->outer) {
+    if (t && t->outer == 1) {
+      t->outer = l->outer, t->s_outer = l->inner * t->s_inner, t->inner = l->inner;   // one stride: any split
+    } else {
+      tokens_kept = tokens.contiguous();
+      t = Lead{l->outer, l->inner, l->inner, 1};
+    }
+  }
+  in.logits = logits.const_data_ptr();
+  in.tokens = tokens_kept.const_data_ptr();
+  in.stride_outer = l->s_outer;
+  in.stride_inner = l->s_inner;
+  in.tok_outer = t->s_outer;
+  in.tok_inner = t->s_inner;
+  in.rows = (uint32_t)tokens.numel();
+  in.inner = (uint32_t)std::max<int64_t>(l->inner, 1);
+  in.vocab = (uint32_t)o.vocab;
+  in.dtype = float_code(logits.scalar_type());
+  in.tokens_i32 = tokens.scalar_type() == at::kInt;
+  in.inv_temp = (float)(1.0 / o.temperature);
+  in.ignore_index = o.ignore_index;
+  return in;
+}
+
+struct LogprobResult { Tensor logprobs, entropy, stats, top_logprobs, top_ids; };
+
+LogprobResult run_logprobs(const Tensor& logits, const Tensor& tokens, const LogprobOptions& o, bool stats) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  LogprobResult r;
+  r.logprobs = at::empty(tokens.sizes(), f32);
+  r.entropy = at::empty(tokens.sizes(), f32);
+  wb::LogprobOut out{};
+  if (stats) {
+    r.stats = at::empty({tokens.numel(), 2}, f32);
+    out.stats = r.stats.mutable_data_ptr<float>();
+  }
+  if (o.top_k) {
+    auto shape = tokens.sizes().vec();
+    shape.push_back(o.top_k);
+    r.top_logprobs = at::empty(shape, f32);
+    r.top_ids = at::empty(shape, f32.dtype(at::kLong));
+    out.top_logprobs = r.top_logprobs.mutable_data_ptr<float>();
+    out.top_ids = r.top_ids.mutable_data_ptr<int64_t>();
+  }
+  out.logprobs = r.logprobs.mutable_data_ptr<float>();
+  out.entropy = r.entropy.mutable_data_ptr<float>();
+  out.top_k = (int)o.top_k;
+  if (tokens.numel() == 0) return r;
+  Tensor kept;
+  const wb::LogprobRows in = rows_of(logits, tokens, o, kept);
+  check(wb::launch_token_logprobs(in, out, c10::cuda::getCurrentCUDAStream()), "token_logprobs launch");
+  return r;
+}
+
+// A gradient over the rows as one stride (autograd hands expanded ones).
+Tensor row_grad(const Tensor& g, const float*& ptr, int64_t& stride) {
+  if (!g.defined()) return g;
+  Tensor t = g.scalar_type() == at::kFloat ? g : g.to(at::kFloat);
+  auto l = lead_of(t, t.dim());
+  if (!l || l->outer != 1) {
+    t = t.contiguous();
+    l = lead_of(t, t.dim());
+  }
+  ptr = t.const_data_ptr<float>();
+  stride = l->s_inner;
+  return t;
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
+                                                int64_t vocab, double temperature, int64_t top_k, int64_t ignore_index) {
+    const LogprobOptions o{vocab, ignore_index, temperature, top_k};
+    LogprobResult r = run_logprobs(logits, tokens, o, true);
+    ctx->save_for_backward({logits, tokens, r.stats, r.entropy});
+    ctx->saved_data["vocab"] = vocab;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->set_materialize_grads(false);
+    if (!top_k) return {r.logprobs, r.entropy};
+    ctx->mark_non_differentiable({r.top_logprobs, r.top_ids});
+    return {r.logprobs, r.entropy, r.top_logprobs, r.top_ids};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (at::GradMode::is_enabled())
+      throw std::runtime_error("token_logprobs: the gradient has no second derivative (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2], &entropy = saved[3];
+    const LogprobOptions o{ctx->saved_data["vocab"].toInt(), ctx->saved_data["ignore_index"].toInt(),
+                           ctx->saved_data["temperature"].toDouble(), 0};
+    const c10::cuda::CUDAGuard guard(logits.device());
+    Tensor grad = at::empty(logits.sizes(), logits.options());
+    if (tokens.numel()) {
+      wb::LogprobGrad g{};
+      const Tensor a = row_grad(grads[0], g.g_logprobs, g.g_logprobs_stride);
+      const Tensor b = row_grad(grads[1], g.g_entropy, g.g_entropy_stride);
+      g.stats = stats.const_data_ptr<float>();
+      g.entropy = entropy.const_data_ptr<float>();
+      g.grad = grad.mutable_data_ptr();
+      g.cols = (uint32_t)logits.size(-1);
+      Tensor kept;
+      const wb::LogprobRows in = rows_of(logits, tokens, o, kept);
+      check(wb::launch_token_logprobs_grad(in, g, c10::cuda::getCurrentCUDAStream()), "token_logprobs gradient launch");
+    }
+    return {grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::optional<int64_t>& columns, double temperature,
+                         int64_t top_k, int64_t ignore_index) {
+  if (logits.dim() < 1) bad("token_logprobs: logits need a vocabulary dimension");
+  const int64_t cols = logits.size(-1), vocab = columns.value_or(cols);
+  if (!float_code(logits.scalar_type())) bad("token_logprobs: logits must be bfloat16, float16 or float32");
+  if (tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) bad("token_logprobs: tokens must be int64 or int32");
+  if (tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+    bad("token_logprobs: tokens of shape " + shape_of(tokens) + " do not match logits of shape " + shape_of(logits));
+  if (vocab < 1 || vocab > cols) bad("token_logprobs: vocab must be between 1 and the logits' " + std::to_string(cols) + " columns");
+  if (cols > std::numeric_limits<int32_t>::max() || tokens.numel() >= std::numeric_limits<int32_t>::max())
+    bad("token_logprobs: at most 2^31 - 1 columns and rows");
+  if (!(temperature > 0) || !std::isfinite(temperature) || !std::isfinite((float)(1.0 / temperature)) || (float)(1.0 / temperature) == 0.f)
+    bad("token_logprobs: the temperature must be positive and finite");
+  if (top_k < 0 || top_k > wb::kLogprobMaxTop || top_k > vocab)
+    bad("token_logprobs: top_k must be between 0 and " + std::to_string(std::min<int64_t>(wb::kLogprobMaxTop, vocab)));
+  if (cols > 1 && logits.stride(-1) != 1) bad("token_logprobs: the logits' last dimension must be contiguous");
+  if (!logits.is_cuda() || !tokens.is_cuda() || logits.device() != tokens.device())
+    bad("token_logprobs: logits and tokens must be CUDA tensors of one device");
+  if (logits.requires_grad() && at::GradMode::is_enabled()) {
+    auto r = TokenLogprobs::apply(logits, tokens, vocab, temperature, top_k, ignore_index);
+    return top_k ? py::make_tuple(r[0], r[1], r[2], r[3]) : py::make_tuple(r[0], r[1], py::none(), py::none());
+  }
+  LogprobResult r = run_logprobs(logits, tokens, {vocab, ignore_index, temperature, top_k}, false);
+  return top_k ? py::make_tuple(r.logprobs, r.entropy, r.top_logprobs, r.top_ids)
+               : py::make_tuple(r.logprobs, r.entropy, py::none(), py::none());
+}
+
+// -- sum of squares, norm -------------------------------------------------------------------------
+// A tensor whose elements fill one stretch of memory without holes, in any order of dimensions.
+bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
+
+py::tuple sum_squares(const std::vector<Tensor>& tensors) {
+  if (tensors.empty()) bad("grad_norm: no tensors");
+  const auto dev = tensors[0].device();
+  std::vector<wb::NormTensor> t;
+  t.reserve(tensors.size());
+  for (const Tensor& x : tensors) {
+    if (!x.is_cuda() || x.device() != dev) bad("grad_norm: all tensors must be CUDA tensors of one device");
+    if (!float_code(x.scalar_type())) bad("grad_norm: tensors must be bfloat16, float16 or float32");
+    if (!dense(x)) bad("grad_norm: a tensor of shape " + shape_of(x) + " has holes or overlaps in memory");
+    if (x.numel()) t.push_back({reinterpret_cast<uint64_t>(x.const_data_ptr()), (uint64_t)x.numel(), float_code(x.scalar_type()), 0});
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  const int sms = sm_count(dev.index());
+  const auto f64 = tensors[0].options().dtype(at::kDouble).requires_grad(false);
+  Tensor sum_sq = at::empty({}, f64), norm = at::empty({}, f64.dtype(at::kFloat));
+  Tensor scratch = at::empty({(int64_t)wb::sum_sq_scratch(t.data(), (uint32_t)t.size(), sms)}, f64);
+  check(wb::launch_sum_sq(t.data(), (uint32_t)t.size(), scratch.mutable_data_ptr<double>(), sum_sq.mutable_data_ptr<double>(),
+                          norm.mutable_data_ptr<float>(), sms, c10::cuda::getCurrentCUDAStream()),
+        "grad_norm launch");
+  return py::make_tuple(sum_sq, norm);
+}
+
+// -- AdamW ----------------------------------------------------------------------------------------
+// The parameters and flat state buffers of one optimizer, its resident tables and its step.
+struct AdamWProgram {
+  std::vector<std::string> names;
+  std::vector<Tensor> params;
+  std::vector<uint64_t> ptrs, offsets;
+  std::vector<float> decay;
+  std::vector<uint32_t> chunk_start;
+  Tensor tables, chunks, clock, m, v, m_scale, v_scale, master;
+  std::vector<uint64_t> grads;
+  int64_t total = 0;
+  double beta1, beta2, eps;
+  bool fp8;
+  at::Device dev{at::kCPU};
+  int sms = 0;
+
+  AdamWProgram(std::vector<std::string> names_, std::vector<Tensor> params_, std::vector<double> decay_, double b1, double b2, double eps_,
+               bool fp8_, bool with_master)
+      : names(std::move(names_)), params(std::move(params_)), beta1(b1), beta2(b2), eps(eps_), fp8(fp8_) {
+    if (params.empty()) bad("AdamW: no parameters");
+    dev = params[0].device();
+    bool narrow = false;
+    uint64_t n_chunks = 0;
+    for (size_t i = 0; i < params.size(); ++i) {
+      check_param(params[i], names[i]);
+      narrow |= params[i].scalar_type() != at::kFloat;
+      offsets.push_back((uint64_t)total);
+      decay.push_back((float)decay_[i]);
+      chunk_start.push_back((uint32_t)n_chunks);
+      n_chunks += ((uint64_t)params[i].numel() + wb::kAdamChunk - 1) / wb::kAdamChunk;
+      total += (params[i].numel() + wb::kStateBlock - 1) / wb::kStateBlock * wb::kStateBlock;
+    }
+    if (n_chunks >= 0x7fffffffull) bad("AdamW: more than 2^31 work items");
+    chunk_start.push_back((uint32_t)n_chunks);
+    if (with_master && !narrow) bad("AdamW: master weights need 16-bit parameters");
+    check_disjoint();
+    const c10::cuda::CUDAGuard guard(dev);
+    sms = sm_count(dev.index());
+    const auto f32 = params[0].options().dtype(at::kFloat).requires_grad(false);
+    if (fp8) {
+      m = at::zeros({total}, f32.dtype(at::kFloat8_e4m3fn));
+      v = at::zeros({total}, f32.dtype(at::kFloat8_e4m3fn));
+      m_scale = at::ones({total / wb::kStateBlock}, f32);
+      v_scale = at::ones({total / wb::kStateBlock}, f32);
+    } else {
+      m = at::zeros({total}, f32);
+      v = at::zeros({total}, f32);
+    }
+    if (with_master) master = at::zeros({total}, f32);
+    clock = at::zeros({(int64_t)sizeof(wb::AdamClock)}, f32.dtype(at::kByte));
+    set_step(0);
+    std::vector<wb::AdamChunk> ch;
+    ch.reserve(n_chunks);
+    for (uint32_t i = 0; i < params.size(); ++i)
+      for (uint32_t c = 0; c < chunk_start[i + 1] - chunk_start[i]; ++c) ch.push_back({i, c});
+    chunks = upload(ch.data(), ch.size() * sizeof(wb::AdamChunk));
+    upload_tensors();
+    if (with_master) read_master();
+    settle();
+  }
+
+  // Tables and states are written on the current stream; steps may run on any other.
+  void settle() const {
+    const c10::cuda::CUDAGuard guard(dev);
+    check(cudaStreamSynchronize(c10::cuda::getCurrentCUDAStream()), "AdamW set-up");
+  }
+
+  void check_param(const Tensor& p, const std::string& name) const {
+    if (!p.is_cuda() || p.device() != dev) bad("AdamW: " + name + " is not on the CUDA device of the first parameter");
+    if (!float_code(p.scalar_type())) bad("AdamW: " + name + " must be bfloat16, float16 or float32");
+    if (!dense(p)) bad("AdamW: " + name + " has holes or overlaps in memory; give the whole parameter, not a view of part of it");
+  }
+
+  void check_disjoint() const {
+    std::vector<std::pair<uint64_t, size_t>> at_;
+    for (size_t i = 0; i < params.size(); ++i)
+      if (params[i].numel()) at_.push_back({reinterpret_cast<uint64_t>(params[i].const_data_ptr()), i});
+    std::sort(at_.begin(), at_.end());
+    for (size_t k = 1; k < at_.size(); ++k)
+      if (at_[k - 1].first + params[at_[k - 1].second].nbytes() > at_[k].first)
+        bad("AdamW: " + names[at_[k - 1].second] + " and " + names[at_[k].second] + " share memory: give a tied parameter once");
+  }
+
+  Tensor upload(const void* p, size_t bytes) const {
+    const c10::cuda::CUDAGuard guard(dev);
+    Tensor host = at::empty({(int64_t)std::max<size_t>(bytes, 16)}, at::TensorOptions().dtype(at::kByte));
+    std::memcpy(host.mutable_data_ptr(), p, bytes);
+    return host.to(dev);
+  }
+
+  void upload_tensors() {
+    std::vector<wb::AdamTensor> t;
+    ptrs.clear();
+    for (size_t i = 0; i < params.size(); ++i) {
+      ptrs.push_back(reinterpret_cast<uint64_t>(params[i].const_data_ptr()));
+      t.push_back({ptrs[i], (uint64_t)params[i].numel(), offsets[i], float_code(params[i].scalar_type()), decay[i]});
+    }
+    tables = upload(t.data(), t.size() * sizeof(wb::AdamTensor));
+  }
+
+  // A tensor's slice of a flat state buffer, in the order of the parameter's memory.
+  Tensor slice(const Tensor& flat, size_t i) const {
+    return at::as_strided(flat, params[i].sizes(), params[i].strides(), (int64_t)offsets[i]);
+  }
+
+  void read_master() {
+    at::NoGradGuard no_grad;
+    for (size_t i = 0; i < params.size(); ++i) slice(master, i).copy_(params[i].detach());
+  }
+
+  void set_step(int64_t step) {
+    wb::AdamClock c{};
+    c.step = step;
+    c.b1t = std::pow(beta1, (double)step);
+    c.b2t = std::pow(beta2, (double)step);
+    Tensor host = at::empty({(int64_t)sizeof(c)}, at::TensorOptions().dtype(at::kByte));
+    std::memcpy(host.mutable_data_ptr(), &c, sizeof(c));
+    clock.copy_(host);
+    settle();
+  }
+
+  int64_t get_step() const {
+    wb::AdamClock c;
+    Tensor host = clock.cpu();
+    std::memcpy(&c, host.const_data_ptr(), sizeof(c));
+    return c.step;
+  }
+
+  // Parameters at new addresses (their memory was released and allocated again).
+  void rebind(const std::vector<Tensor>& p) {
+    if (p.size() != params.size()) bad("AdamW.rebind: another number of parameters");
+    for (size_t i = 0; i < p.size(); ++i) {
+      check_param(p[i], names[i]);
+      if (p[i].sizes() != params[i].sizes() || p[i].strides() != params[i].strides() || p[i].scalar_type() != params[i].scalar_type())
+        bad("AdamW.rebind: " + names[i] + " has another shape, stride or type");
+    }
+    auto before = params;
+    params = p;
+    try {
+      check_disjoint();
+    } catch (...) {
+      params = before;
+      throw;
+    }
+    const c10::cuda::CUDAGuard guard(dev);
+    check(cudaDeviceSynchronize(), "AdamW.rebind");       // steps in flight on any stream read the old table
+    upload_tensors();
+    settle();
+  }
+
+  // Collects the gradients of this step; `given`: those that are there, for the norm.
+  void collect(const py::object& src, std::vector<Tensor>* given) {
+    grads.assign(params.size(), 0);
+    Py_ssize_t found = 0;
+    const bool dict = !src.is_none();
+    if (dict && !PyDict_Check(src.ptr())) throw py::type_error("AdamW.step: gradients are a dict of name -> tensor, or None for the parameters' .grad");
+    for (size_t i = 0; i < params.size(); ++i) {
+      if (reinterpret_cast<uint64_t>(params[i].const_data_ptr()) != ptrs[i])
+        throw std::runtime_error("AdamW.step: " + names[i] + " moved in memory; call rebind()");
+      Tensor g;
+      if (dict) {
+        PyObject* o = PyDict_GetItemWithError(src.ptr(), py_names[i].ptr());
+        if (!o && PyErr_Occurred()) throw py::error_already_set();
+        if (o) {
+          ++found;
+          if (o != Py_None) {
+            if (!THPVariable_Check(o)) throw py::type_error("AdamW.step: the gradient of " + names[i] + " is not a tensor");
+            g = THPVariable_Unpack(o);
+          }
+        }
+      } else {
+        g = params[i].grad();
+      }
+      if (!g.defined()) continue;
+      const Tensor& p = params[i];
+      if (!g.is_cuda() || g.device() != dev) bad("AdamW.step: the gradient of " + names[i] + " is on another device");
+      if (g.sizes() != p.sizes()) bad("AdamW.step: the gradient of " + names[i] + " has shape " + shape_of(g) + ", not " + shape_of(p));
+      if (g.scalar_type() != p.scalar_type() && g.scalar_type() != at::kFloat)
+        bad("AdamW.step: the gradient of " + names[i] + " must have the parameter's type or float32");
+      if (g.strides() != p.strides() && !same_order(g, p))
+        bad("AdamW.step: the gradient of " + names[i] + " has another memory layout than the parameter");
+      if (!g.numel()) continue;
+      grads[i] = reinterpret_cast<uint64_t>(g.const_data_ptr()) | (g.scalar_type() != p.scalar_type() ? 1u : 0u);
+      if (given) given->push_back(g);
+    }
+    if (dict && found != PyDict_Size(src.ptr())) bad("AdamW.step: the gradients name a tensor that is not one of the parameters");
+  }
+
+  // Strides may differ in dimensions of size 1.
+  static bool same_order(const Tensor& g, const Tensor& p) {
+    for (int64_t d = 0; d < p.dim(); ++d)
+      if (p.size(d) != 1 && g.stride(d) != p.stride(d)) return false;
+    return true;
+  }
+
+  std::vector<py::str> py_names;
+
+  // The sum of squares of this step's gradients (before a reduction over ranks), or None without any.
+  py::object grad_sum_sq(const py::object& src) {
+    std::vector<Tensor> given;
+    collect(src, &given);
+    if (given.empty()) return py::none();
+    return sum_squares(given)[0];
+  }
+
+  py::object step(const py::object& src, double lr, const std::optional<Tensor>& lr_dev, const std::optional<Tensor>& sum_sq, double max_norm) {
+    collect(src, nullptr);
+    const c10::cuda::CUDAGuard guard(dev);
+    wb::AdamArgs a{};
+    if (lr_dev) {
+      if (lr_dev->numel() != 1 || lr_dev->device() != dev || (lr_dev->scalar_type() != at::kFloat && lr_dev->scalar_type() != at::kDouble))
+        bad("AdamW.step: lr is a number, or a float32 or float64 tensor of one element on the parameters' device");
+      a.lr_ptr = lr_dev->const_data_ptr();
+      a.lr_f64 = lr_dev->scalar_type() == at::kDouble;
+    }
+    Tensor norm;
+    if (sum_sq) {
+      if (sum_sq->numel() != 1 || sum_sq->device() != dev || sum_sq->scalar_type() != at::kDouble) bad("AdamW.step: bad sum of squares");
+      norm = at::empty({}, m_options());
+      a.sum_sq = sum_sq->const_data_ptr<double>();
+      a.norm = norm.mutable_data_ptr<float>();
+    }
+    a.tensors = reinterpret_cast<const wb::AdamTensor*>(tables.const_data_ptr());
+    a.chunks = reinterpret_cast<const wb::AdamChunk*>(chunks.const_data_ptr());
+    a.n_tensors = (uint32_t)params.size();
+    a.master = master.defined() ? master.mutable_data_ptr<float>() : nullptr;
+    a.m = m.mutable_data_ptr();
+    a.v = v.mutable_data_ptr();
+    a.m_scale = fp8 ? m_scale.mutable_data_ptr<float>() : nullptr;
+    a.v_scale = fp8 ? v_scale.mutable_data_ptr<float>() : nullptr;
+    a.clock = reinterpret_cast<wb::AdamClock*>(clock.mutable_data_ptr());
+    a.beta1 = beta1;
+    a.beta2 = beta2;
+    a.lr = lr;
+    a.eps = eps;
+    a.max_norm = max_norm;
+    check(wb::launch_adamw(a, grads.data(), chunk_start.data(), sms, c10::cuda::getCurrentCUDAStream()), "AdamW launch");
+    for (const Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();
+    return norm.defined() ? py::cast(norm) : py::none();
+  }
+
+  at::TensorOptions m_options() const { return params[0].options().dtype(at::kFloat).requires_grad(false); }
+};
+
+}  // namespace
+
+namespace wb {
+
+void bind_learn(py::module_& m) {
+  m.def("token_logprobs", &token_logprobs, "log probabilities of tokens, entropy and alternatives");
+  m.def("sum_squares", &sum_squares, "sum of squares of many tensors and its root (device scalars)");
+  py::class_<AdamWProgram>(m, "AdamWProgram")
+      .def(py::init([](std::vector<std::string> names, std::vector<Tensor> params, std::vector<double> decay, double b1, double b2,
+                       double eps, bool fp8, bool master) {
+        if (names.size() != params.size() || names.size() != decay.size()) bad("AdamW: names, parameters and decays must match");
+        auto p = std::make_unique<AdamWProgram>(std::move(names), std::move(params), std::move(decay), b1, b2, eps, fp8, master);
+        for (const auto& n : p->names) p->py_names.emplace_back(n);
+        return p;
+      }))
+      .def("step", &AdamWProgram::step)
+      .def("grad_sum_sq", &AdamWProgram::grad_sum_sq)
+      .def("rebind", &AdamWProgram::rebind)
+      .def("read_master", &AdamWProgram::read_master)
+      .def("slice", [](const AdamWProgram& p, const Tensor& flat, size_t i) { return p.slice(flat, i); })
+      .def_property("step_count", &AdamWProgram::get_step, &AdamWProgram::set_step)
+      .def_readonly("total", &AdamWProgram::total)
+      .def_readonly("exp_avg", &AdamWProgram::m)
+      .def_readonly("second", &AdamWProgram::v)
+      .def_readonly("exp_avg_scale", &AdamWProgram::m_scale)
+      .def_readonly("second_scale", &AdamWProgram::v_scale)
+      .def_readonly("master", &AdamWProgram::master);
+}
+
+}  // namespace wb

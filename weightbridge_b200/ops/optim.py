@@ -1,0 +1,153 @@
+"""The optimizer step that produces the weights a sync sends: AdamW over many tensors in one
+launch, with states in 32 or 8 bits, and the global gradient norm.
+"""
+from __future__ import annotations
+
+from typing import Any, Callable, Iterable, Mapping
+
+import torch
+
+from ._ext import ext
+
+STATE_BLOCK = 128           # elements that share a scale in the 8-bit states
+
+
+def grad_norm(tensors: Mapping[str, torch.Tensor] | Iterable[torch.Tensor], group: Any = None) -> torch.Tensor:
+    """The 2-norm over all ``tensors`` (a dict or an iterable; ``None`` entries are left out) as
+    an fp32 scalar on their device, without waiting for it.
+
+    bf16, fp16 and fp32 tensors of one device, each filling its memory without holes.  The sum
+    runs in a fixed order: the same inputs give the same bits.  ``group``: a process group over
+    which the squares are summed; a tensor that several of its ranks hold counts once per rank.
+    Squares are formed in 32 bits: a gradient above 1.8e19 makes the norm infinite.
+    """
+    ts = [t for t in (tensors.values() if isinstance(tensors, Mapping) else tensors) if t is not None]
+    sum_sq, norm = ext().sum_squares(ts)
+    if group is None:
+        return norm
+    torch.distributed.all_reduce(sum_sq, group=group)
+    return sum_sq.sqrt().float()
+
+
+class AdamW:
+    """AdamW (decoupled weight decay) over a dict of tensors, one launch per step.
+
+    ``params``: name -> tensor, e.g. ``dict(model.named_parameters())`` or the tensors a layout
+    allocates; bf16, fp16 or fp32 on one CUDA device, each filling its memory without holes (any
+    order of dimensions).  They are updated in place.  ``states``: ``"fp32"``, or ``"fp8"``:
+    both moments as e4m3 with one fp32 scale per 128 elements, 2.06 bytes a parameter instead of
+    8 (the second moment as its root).  An 8-bit second moment follows changes of a few percent a
+    step only through its block's largest element: use a ``beta2`` of at most 0.99 with it.
+    ``master``: keep fp32 master weights of 16-bit parameters (taken from the parameters now);
+    without them an update below half a step of the 16-bit type is lost.  ``no_decay``: names
+    without weight decay, or a function of the name.
+
+    The states are flat buffers (``states()``); every tensor's slice starts at a multiple of 128
+    elements, in the order of ``params``.  The step count lives on the device, so a captured step
+    can be replayed.
+    """
+
+    def __init__(self, params: Mapping[str, torch.Tensor], lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 0.01, *, states: str = "fp32", master: bool = False,
+                 no_decay: Iterable[str] | Callable[[str], bool] = ()):
+        if states not in ("fp32", "fp8"):
+            raise ValueError(f"AdamW: states must be 'fp32' or 'fp8', not {states!r}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"AdamW: betas must be in [0, 1), not {betas}")
+        if not eps > 0.0 or not weight_decay >= 0.0:
+            raise ValueError("AdamW: eps must be positive and weight_decay not negative")
+        self._check_lr(lr)
+        self.lr = lr
+        self.betas, self.eps, self.weight_decay = tuple(map(float, betas)), float(eps), float(weight_decay)
+        self.state_bits = states
+        self.names = list(params)
+        skip = no_decay if callable(no_decay) else frozenset(no_decay).__contains__
+        if not callable(no_decay) and (unknown := frozenset(no_decay) - set(self.names)):
+            raise ValueError(f"AdamW: no_decay names {sorted(unknown)[0]!r}, which is not a parameter")
+        self._program = ext().AdamWProgram(self.names, list(params.values()), [0.0 if skip(n) else self.weight_decay for n in self.names],
+                                           *self.betas, self.eps, states == "fp8", bool(master))
+
+    @staticmethod
+    def _check_lr(lr) -> None:
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"AdamW: lr must not be negative, not {lr}")
+
+    def step(self, grads: Mapping[str, torch.Tensor] | None = None, *, lr: float | torch.Tensor | None = None,
+             max_norm: float | None = None, group: Any = None) -> torch.Tensor | None:
+        """One update from ``grads`` (name -> tensor of the parameter's type or fp32; default: the
+        parameters' ``.grad``).  A parameter without a gradient is left alone in this step.
+
+        ``lr``: this step's learning rate (default: ``self.lr``); a one-element tensor on the
+        device is read there, so that it can change under a captured step.  ``max_norm``: scale
+        the gradients by ``min(1, max_norm / (norm + 1e-6))``; the global norm is returned as a
+        device scalar, and a step whose norm is not finite changes nothing, nor the step count.
+        ``group``: the ranks whose squares make up the norm (``grad_norm``).  Nothing waits for
+        the GPU.
+        """
+        p = self._program
+        lr = self.lr if lr is None else lr
+        self._check_lr(lr)
+        on_device = lr if isinstance(lr, torch.Tensor) else None
+        number = 0.0 if on_device is not None else float(lr)
+        if max_norm is None:
+            return p.step(grads, number, on_device, None, 0.0)
+        if not max_norm > 0.0:
+            raise ValueError(f"AdamW.step: max_norm must be positive, not {max_norm}")
+        sum_sq = p.grad_sum_sq(grads)
+        if group is not None:
+            if sum_sq is None:                  # a rank without gradients still takes part in the reduction
+                sum_sq = torch.zeros((), dtype=torch.float64, device=p.exp_avg.device)
+            torch.distributed.all_reduce(sum_sq, group=group)
+        return p.step(grads, number, on_device, sum_sq, float(max_norm))
+
+    def states(self) -> dict[str, torch.Tensor]:
+        """The flat state buffers: ``exp_avg`` and ``exp_avg_sq`` (fp32), or ``exp_avg`` and
+        ``rms`` (e4m3, the root of the second moment) with ``exp_avg_scale`` and ``rms_scale``;
+        ``master`` with master weights.  They are the optimizer's own, not copies."""
+        p = self._program
+        if self.state_bits == "fp8":
+            out = {"exp_avg": p.exp_avg, "exp_avg_scale": p.exp_avg_scale, "rms": p.second, "rms_scale": p.second_scale}
+        else:
+            out = {"exp_avg": p.exp_avg, "exp_avg_sq": p.second}
+        if p.master is not None:
+            out["master"] = p.master
+        return out
+
+    def slices(self, flat: torch.Tensor) -> dict[str, torch.Tensor]:
+        """Every parameter's slice of a flat buffer of ``states()``, shaped like the parameter."""
+        if flat.numel() != self._program.total:
+            raise ValueError("AdamW.slices: not a buffer of one value per element")
+        return {n: self._program.slice(flat, i) for i, n in enumerate(self.names)}
+
+    @property
+    def step_count(self) -> int:
+        """How many updates were taken (reads the device)."""
+        return self._program.step_count
+
+    def rebind(self, params: Mapping[str, torch.Tensor]) -> None:
+        """Go on with the same parameters at new addresses (their memory was released and
+        allocated again, e.g. by an engine that shares the GPU)."""
+        if list(params) != self.names:
+            raise ValueError("AdamW.rebind: the parameters' names or their order differ")
+        self._program.rebind(list(params.values()))
+
+    def state_dict(self) -> dict:
+        """The step count, the names and the state buffers (not copies)."""
+        return {"step": self.step_count, "names": list(self.names), **self.states()}
+
+    def load_state_dict(self, saved: Mapping[str, Any]) -> None:
+        """Take over the states of ``saved`` (of an optimizer of the same parameters and state
+        bits); with master weights, the parameters keep their values until the next step."""
+        if list(saved["names"]) != self.names:
+            raise ValueError("AdamW.load_state_dict: the parameters' names or their order differ")
+        own = self.states()
+        for name, buf in own.items():
+            src = saved.get(name)
+            if src is None or src.shape != buf.shape or src.dtype != buf.dtype:
+                raise ValueError(f"AdamW.load_state_dict: {name} is missing or of another size or type")
+        if int(saved["step"]) < 0:
+            raise ValueError("AdamW.load_state_dict: the step count is negative")
+        for name, buf in own.items():
+            if buf.data_ptr() != saved[name].data_ptr():
+                buf.copy_(saved[name])
+        self._program.step_count = int(saved["step"])
