@@ -144,7 +144,7 @@ LogprobResult run_logprobs(const Tensor& logits, const Tensor& tokens, const Log
   if (tokens.numel() == 0) return r;
   Tensor kept;
   const wb::LogprobRows in = rows_of(logits, tokens, o, kept);
-  check(wb::launch_token_logprobs(in, out, c10::cuda::getCurrentCUDAStream()), "token_logprobs launch");
+  check(wb::launch_token_logprobs(in, out, sm_count(logits.device().index()), c10::cuda::getCurrentCUDAStream()), "token_logprobs launch");
   return r;
 }
 
@@ -217,6 +217,8 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::
     bad("token_logprobs: the temperature must be positive and finite");
   if (top_k < 0 || top_k > wb::kLogprobMaxTop || top_k > vocab)
     bad("token_logprobs: top_k must be between 0 and " + std::to_string(std::min<int64_t>(wb::kLogprobMaxTop, vocab)));
+  if (top_k && vocab > wb::kLogprobMaxTopVocab)
+    bad("token_logprobs: alternatives (top_k) of at most " + std::to_string(wb::kLogprobMaxTopVocab) + " columns");
   if (cols > 1 && logits.stride(-1) != 1) bad("token_logprobs: the logits' last dimension must be contiguous");
   if (!logits.is_cuda() || !tokens.is_cuda() || logits.device() != tokens.device())
     bad("token_logprobs: logits and tokens must be CUDA tensors of one device");
@@ -233,6 +235,19 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::
 // A tensor whose elements fill one stretch of memory without holes, in any order of dimensions.
 bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
 
+// Partial sums of squares of tensors that were checked; `dev`: where they are.
+Tensor partial_sums(std::vector<wb::NormTensor>& t, const at::TensorOptions& f64, int sms) {
+  Tensor partial = at::empty({(int64_t)std::max<uint64_t>(wb::partial_sums_size((uint32_t)t.size(), sms), 1)}, f64);
+  uint32_t n = 0;
+  check(wb::launch_partial_sums(t.data(), (uint32_t)t.size(), partial.mutable_data_ptr<double>(), &n, sms, c10::cuda::getCurrentCUDAStream()),
+        "gradient norm launch");
+  return partial.narrow(0, 0, n);
+}
+
+wb::NormTensor norm_tensor(const Tensor& x) {
+  return {reinterpret_cast<uint64_t>(x.const_data_ptr()), (uint64_t)x.numel(), float_code(x.scalar_type()), 0};
+}
+
 py::tuple sum_squares(const std::vector<Tensor>& tensors) {
   if (tensors.empty()) bad("grad_norm: no tensors");
   const auto dev = tensors[0].device();
@@ -242,15 +257,14 @@ py::tuple sum_squares(const std::vector<Tensor>& tensors) {
     if (!x.is_cuda() || x.device() != dev) bad("grad_norm: all tensors must be CUDA tensors of one device");
     if (!float_code(x.scalar_type())) bad("grad_norm: tensors must be bfloat16, float16 or float32");
     if (!dense(x)) bad("grad_norm: a tensor of shape " + shape_of(x) + " has holes or overlaps in memory");
-    if (x.numel()) t.push_back({reinterpret_cast<uint64_t>(x.const_data_ptr()), (uint64_t)x.numel(), float_code(x.scalar_type()), 0});
+    if (x.numel()) t.push_back(norm_tensor(x));
   }
   const c10::cuda::CUDAGuard guard(dev);
-  const int sms = sm_count(dev.index());
   const auto f64 = tensors[0].options().dtype(at::kDouble).requires_grad(false);
+  const Tensor partial = partial_sums(t, f64, sm_count(dev.index()));
   Tensor sum_sq = at::empty({}, f64), norm = at::empty({}, f64.dtype(at::kFloat));
-  Tensor scratch = at::empty({(int64_t)wb::sum_sq_scratch(t.data(), (uint32_t)t.size(), sms)}, f64);
-  check(wb::launch_sum_sq(t.data(), (uint32_t)t.size(), scratch.mutable_data_ptr<double>(), sum_sq.mutable_data_ptr<double>(),
-                          norm.mutable_data_ptr<float>(), sms, c10::cuda::getCurrentCUDAStream()),
+  check(wb::launch_norm(partial.const_data_ptr<double>(), (uint32_t)partial.numel(), sum_sq.mutable_data_ptr<double>(),
+                        norm.mutable_data_ptr<float>(), c10::cuda::getCurrentCUDAStream()),
         "grad_norm launch");
   return py::make_tuple(sum_sq, norm);
 }
@@ -266,6 +280,7 @@ struct AdamWProgram {
   Tensor tables, chunks, clock, m, v, m_scale, v_scale, master;
   std::vector<uint64_t> grads;
   int64_t total = 0;
+  uint32_t chunk = wb::kAdamTile;
   double beta1, beta2, eps;
   bool fp8;
   at::Device dev{at::kCPU};
@@ -283,16 +298,21 @@ struct AdamWProgram {
       narrow |= params[i].scalar_type() != at::kFloat;
       offsets.push_back((uint64_t)total);
       decay.push_back((float)decay_[i]);
-      chunk_start.push_back((uint32_t)n_chunks);
-      n_chunks += ((uint64_t)params[i].numel() + wb::kAdamChunk - 1) / wb::kAdamChunk;
       total += (params[i].numel() + wb::kStateBlock - 1) / wb::kStateBlock * wb::kStateBlock;
     }
-    if (n_chunks >= 0x7fffffffull) bad("AdamW: more than 2^31 work items");
+    const c10::cuda::CUDAGuard guard(dev);
+    sms = sm_count(dev.index());
+    // A work item: four tiles where the SMs still get eight items each, which reads a tensor's entry
+    // once for all four; one tile for small models, where it takes many CTAs to fill the GPU at all.
+    chunk = total >= (int64_t)sms * 8 * 4 * wb::kAdamTile ? 4 * wb::kAdamTile : wb::kAdamTile;
+    for (const Tensor& p : params) {
+      chunk_start.push_back((uint32_t)n_chunks);
+      n_chunks += ((uint64_t)p.numel() + chunk - 1) / chunk;
+      if (n_chunks >= 0x7fffffffull) bad("AdamW: too many elements");
+    }
     chunk_start.push_back((uint32_t)n_chunks);
     if (with_master && !narrow) bad("AdamW: master weights need 16-bit parameters");
     check_disjoint();
-    const c10::cuda::CUDAGuard guard(dev);
-    sms = sm_count(dev.index());
     const auto f32 = params[0].options().dtype(at::kFloat).requires_grad(false);
     if (fp8) {
       m = at::zeros({total}, f32.dtype(at::kFloat8_e4m3fn));
@@ -405,16 +425,17 @@ struct AdamWProgram {
     settle();
   }
 
-  // Collects the gradients of this step; `given`: those that are there, for the norm.
-  void collect(const py::object& src, std::vector<Tensor>* given) {
+  // Collects the gradients of this step, and what the norm reads of them.
+  void collect(const py::object& src, std::vector<wb::NormTensor>* normed) {
     grads.assign(params.size(), 0);
     Py_ssize_t found = 0;
     const bool dict = !src.is_none();
     if (dict && !PyDict_Check(src.ptr())) throw py::type_error("AdamW.step: gradients are a dict of name -> tensor, or None for the parameters' .grad");
     for (size_t i = 0; i < params.size(); ++i) {
-      if (reinterpret_cast<uint64_t>(params[i].const_data_ptr()) != ptrs[i])
+      const Tensor& p = params[i];
+      if (reinterpret_cast<uint64_t>(p.const_data_ptr()) != ptrs[i])
         throw std::runtime_error("AdamW.step: " + names[i] + " moved in memory; call rebind()");
-      Tensor g;
+      const Tensor* g = nullptr;
       if (dict) {
         PyObject* o = PyDict_GetItemWithError(src.ptr(), py_names[i].ptr());
         if (!o && PyErr_Occurred()) throw py::error_already_set();
@@ -422,23 +443,22 @@ struct AdamWProgram {
           ++found;
           if (o != Py_None) {
             if (!THPVariable_Check(o)) throw py::type_error("AdamW.step: the gradient of " + names[i] + " is not a tensor");
-            g = THPVariable_Unpack(o);
+            g = &THPVariable_Unpack(o);
           }
         }
       } else {
-        g = params[i].grad();
+        g = &p.grad();
       }
-      if (!g.defined()) continue;
-      const Tensor& p = params[i];
-      if (!g.is_cuda() || g.device() != dev) bad("AdamW.step: the gradient of " + names[i] + " is on another device");
-      if (g.sizes() != p.sizes()) bad("AdamW.step: the gradient of " + names[i] + " has shape " + shape_of(g) + ", not " + shape_of(p));
-      if (g.scalar_type() != p.scalar_type() && g.scalar_type() != at::kFloat)
+      if (!g || !g->defined()) continue;
+      if (!g->is_cuda() || g->device() != dev) bad("AdamW.step: the gradient of " + names[i] + " is on another device");
+      if (g->sizes() != p.sizes()) bad("AdamW.step: the gradient of " + names[i] + " has shape " + shape_of(*g) + ", not " + shape_of(p));
+      if (g->scalar_type() != p.scalar_type() && g->scalar_type() != at::kFloat)
         bad("AdamW.step: the gradient of " + names[i] + " must have the parameter's type or float32");
-      if (g.strides() != p.strides() && !same_order(g, p))
+      if (g->strides() != p.strides() && !same_order(*g, p))
         bad("AdamW.step: the gradient of " + names[i] + " has another memory layout than the parameter");
-      if (!g.numel()) continue;
-      grads[i] = reinterpret_cast<uint64_t>(g.const_data_ptr()) | (g.scalar_type() != p.scalar_type() ? 1u : 0u);
-      if (given) given->push_back(g);
+      if (!g->numel()) continue;
+      grads[i] = reinterpret_cast<uint64_t>(g->const_data_ptr()) | (g->scalar_type() != p.scalar_type() ? 1u : 0u);
+      if (normed) normed->push_back(norm_tensor(*g));
     }
     if (dict && found != PyDict_Size(src.ptr())) bad("AdamW.step: the gradients name a tensor that is not one of the parameters");
   }
@@ -452,16 +472,26 @@ struct AdamWProgram {
 
   std::vector<py::str> py_names;
 
-  // The sum of squares of this step's gradients (before a reduction over ranks), or None without any.
-  py::object grad_sum_sq(const py::object& src) {
-    std::vector<Tensor> given;
-    collect(src, &given);
-    if (given.empty()) return py::none();
-    return sum_squares(given)[0];
+  // The sum of squares of this step's gradients, before a reduction over ranks.
+  Tensor grad_sum_sq(const py::object& src) {
+    std::vector<wb::NormTensor> t;
+    collect(src, &t);
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto f64 = f32_options().dtype(at::kDouble);
+    const Tensor partial = partial_sums(t, f64, sms);
+    Tensor sum_sq = at::empty({}, f64), norm = at::empty({}, f32_options());
+    check(wb::launch_norm(partial.const_data_ptr<double>(), (uint32_t)partial.numel(), sum_sq.mutable_data_ptr<double>(),
+                          norm.mutable_data_ptr<float>(), c10::cuda::getCurrentCUDAStream()),
+          "gradient norm launch");
+    return sum_sq;
   }
 
+  // max_norm > 0: clip, by the given sum of squares or by these gradients' own.
   py::object step(const py::object& src, double lr, const std::optional<Tensor>& lr_dev, const std::optional<Tensor>& sum_sq, double max_norm) {
-    collect(src, nullptr);
+    const bool clip = max_norm > 0;
+    std::vector<wb::NormTensor> t;
+    if (clip && !sum_sq) t.reserve(params.size());
+    collect(src, clip && !sum_sq ? &t : nullptr);
     const c10::cuda::CUDAGuard guard(dev);
     wb::AdamArgs a{};
     if (lr_dev) {
@@ -470,16 +500,19 @@ struct AdamWProgram {
       a.lr_ptr = lr_dev->const_data_ptr();
       a.lr_f64 = lr_dev->scalar_type() == at::kDouble;
     }
-    Tensor norm;
-    if (sum_sq) {
-      if (sum_sq->numel() != 1 || sum_sq->device() != dev || sum_sq->scalar_type() != at::kDouble) bad("AdamW.step: bad sum of squares");
-      norm = at::empty({}, m_options());
-      a.sum_sq = sum_sq->const_data_ptr<double>();
+    Tensor norm, partial;
+    if (clip) {
+      if (sum_sq) partial = *sum_sq;
+      else partial = partial_sums(t, f32_options().dtype(at::kDouble), sms);
+      norm = at::empty({}, f32_options());
+      a.partial = partial.const_data_ptr<double>();
+      a.n_partial = (uint32_t)partial.numel();
       a.norm = norm.mutable_data_ptr<float>();
     }
     a.tensors = reinterpret_cast<const wb::AdamTensor*>(tables.const_data_ptr());
     a.chunks = reinterpret_cast<const wb::AdamChunk*>(chunks.const_data_ptr());
     a.n_tensors = (uint32_t)params.size();
+    a.chunk = chunk;
     a.master = master.defined() ? master.mutable_data_ptr<float>() : nullptr;
     a.m = m.mutable_data_ptr();
     a.v = v.mutable_data_ptr();
@@ -496,7 +529,7 @@ struct AdamWProgram {
     return norm.defined() ? py::cast(norm) : py::none();
   }
 
-  at::TensorOptions m_options() const { return params[0].options().dtype(at::kFloat).requires_grad(false); }
+  at::TensorOptions f32_options() const { return params[0].options().dtype(at::kFloat).requires_grad(false); }
 };
 
 }  // namespace

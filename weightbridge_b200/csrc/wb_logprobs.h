@@ -8,6 +8,7 @@
 namespace wb {
 
 constexpr int kLogprobMaxTop = 32;
+constexpr uint32_t kLogprobMaxTopVocab = 1u << 22;     // columns with alternatives: the tiles' maxima fit shared memory
 
 // Rows of logits: row r = (r / inner, r % inner) starts at element (r / inner) * stride_outer +
 // (r % inner) * stride_inner; its columns are contiguous.  The same split addresses the tokens.
@@ -43,7 +44,7 @@ struct LogprobGrad {
   uint32_t cols;               // >= vocab; columns past the vocabulary get zeros
 };
 
-cudaError_t launch_token_logprobs(const LogprobRows& in, const LogprobOut& out, cudaStream_t stream);
+cudaError_t launch_token_logprobs(const LogprobRows& in, const LogprobOut& out, int sms, cudaStream_t stream);
 cudaError_t launch_token_logprobs_grad(const LogprobRows& in, const LogprobGrad& g, cudaStream_t stream);
 
 }  // namespace wb

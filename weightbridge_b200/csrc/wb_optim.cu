@@ -13,14 +13,16 @@
 // without bound, a denominator rounded up only shortens it.
 #include "wb_optim.h"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+#include "wb_vec.cuh"
 
 namespace wb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr double kMaxDouble = 1.7976931348623157e308;
 
 __device__ __forceinline__ float load_as_f32(uint64_t p, uint32_t dtype, uint64_t i) {
   if (dtype == DT_F32) return reinterpret_cast<const float*>(p)[i];
@@ -34,11 +36,18 @@ __device__ __forceinline__ void store_from_f32(uint64_t p, uint32_t dtype, uint6
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
 }
 
-__device__ __forceinline__ float e4m3_to_f32(uint8_t q) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(q, __NV_E4M3)));
+// A sum over the CTA in a fixed order; all threads get it.
+__device__ __forceinline__ double cta_sum(double v, double* red) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < kWarps; ++i) v += red[i];
+  return v;
 }
 
-struct StepScalars { float b1, om_b1, b2, om_b2, step_size, inv_c2, eps, coef; double lr; };
+// -- the step -------------------------------------------------------------------------------------
+struct StepScalars { float b1, om_b1, b2, om_b2, step_size, root_c2, eps, coef, lr; };
 
 template <int N>
 struct Grads {
@@ -46,10 +55,41 @@ struct Grads {
   uint32_t first_tensor, first_chunk, n_chunks, last;
 };
 
-__device__ __forceinline__ float warp_max(float v) {
+__device__ __forceinline__ float root(float x) {          // relative error 2^-23
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// One element: the new moments, the new value and r = sqrt(v).
+__device__ __forceinline__ void update(const StepScalars& s, float keep, float grad, float& m, float& v, float& p, float& r) {
+  const float g = grad * s.coef;
+  m = s.b1 * m + s.om_b1 * g;
+  v = s.b2 * v + s.om_b2 * g * g;
+  r = root(v);
+  p = p * keep - s.step_size * __fdividef(m, r * s.root_c2 + s.eps);
+}
+
+__device__ __forceinline__ float2 decode2(uint32_t q) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q & 0xffffu), __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+
+__device__ __forceinline__ void decode8(uint2 q, float scale, float (&x)[8]) {
+  const uint32_t w[4] = {q.x, q.x >> 16, q.y, q.y >> 16};
   #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  return v;
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = decode2(w[i]);
+    x[2 * i] = f.x * scale;
+    x[2 * i + 1] = f.y * scale;
+  }
+}
+
+__device__ __forceinline__ uint2 encode8(const float (&x)[8]) {
+  uint32_t w[4];
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 
 // scale of a block; tiny blocks keep a normal scale, whose reciprocal is finite
@@ -57,93 +97,178 @@ __device__ __forceinline__ float block_scale(float amax) {
   return amax > 0.f ? fmaxf(__fdiv_rn(amax, kE4M3Max), 1.17549435e-38f) : 1.f;
 }
 
+// r / scale, where a positive r keeps at least the smallest code
+__device__ __forceinline__ float root_code(float r, float inv) { return fmaxf(r * inv, r > 0.f ? 0.001953125f : 0.f); }
+
+// 256 elements from element i0 of the tensor on, eight a lane, all addresses aligned to eight
+// elements: 16 lanes hold a block of the 8-bit states.
+template <bool FP8, typename P, typename G>
+__device__ __forceinline__ void step_vector(const AdamArgs& a, const StepScalars& s, float keep, P* param, const G* grad, uint64_t si) {
+  float g[8], m[8], v[8], p[8], r[8];
+  load_eight(grad, g);
+  const uint64_t blk = si / kStateBlock;
+  float ms = 0.f, rs = 0.f;
+  uint2 mq, rq;
+  if constexpr (FP8) {
+    mq = load8(reinterpret_cast<const uint8_t*>(a.m) + si);
+    rq = load8(reinterpret_cast<const uint8_t*>(a.v) + si);
+    ms = a.m_scale[blk];
+    rs = a.v_scale[blk];
+  } else {
+    load_eight(reinterpret_cast<const float*>(a.m) + si, m);
+    load_eight(reinterpret_cast<const float*>(a.v) + si, v);
+  }
+  if (a.master) load_eight(a.master + si, p);
+  else load_eight(param, p);
+  if constexpr (FP8) {
+    decode8(mq, ms, m);
+    decode8(rq, rs, v);
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= v[i];
+  }
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) update(s, keep, g[i], m[i], v[i], p[i], r[i]);
+  if (a.master) store_eight(a.master + si, p);
+  store_eight(param, p);
+  if constexpr (FP8) {
+    float ma = 0.f, ra = 0.f;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) ma = fmaxf(ma, fabsf(m[i])), ra = fmaxf(ra, r[i]);
+    #pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      ma = fmaxf(ma, __shfl_xor_sync(kFullWarp, ma, o));
+      ra = fmaxf(ra, __shfl_xor_sync(kFullWarp, ra, o));
+    }
+    ms = block_scale(ma);
+    rs = block_scale(ra);
+    const float mi = __frcp_rn(ms), ri = __frcp_rn(rs);
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] *= mi, r[i] = root_code(r[i], ri);
+    store8(reinterpret_cast<uint8_t*>(a.m) + si, encode8(m));
+    store8(reinterpret_cast<uint8_t*>(a.v) + si, encode8(r));
+    if ((threadIdx.x & 15) == 0) {        // the lanes' shuffles came after their loads of the old scales
+      a.m_scale[blk] = ms;
+      a.v_scale[blk] = rs;
+    }
+  } else {
+    store_eight(reinterpret_cast<float*>(a.m) + si, m);
+    store_eight(reinterpret_cast<float*>(a.v) + si, v);
+  }
+}
+
+// One block of 128 elements, or what is left of the tensor: single elements side by side, four a
+// lane, for tensors at odd addresses and for their ends.
+template <bool FP8>
+__device__ __forceinline__ void step_block(const AdamArgs& a, const StepScalars& s, float keep, const AdamTensor& t, uint64_t grad,
+                                           uint32_t gtype, uint64_t b, uint64_t end) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t blk = (t.state + b) / kStateBlock;
+  float m[4], v[4], r[4], p[4], g[4], ms = 0.f, rs = 0.f;
+  if constexpr (FP8) ms = a.m_scale[blk], rs = a.v_scale[blk];
+  #pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint64_t i = b + lane + 32 * k, si = t.state + i;
+    m[k] = v[k] = g[k] = p[k] = 0.f;
+    if (i >= end) continue;
+    g[k] = load_as_f32(grad, gtype, i);
+    if constexpr (FP8) {
+      m[k] = decode2(reinterpret_cast<const uint8_t*>(a.m)[si]).x * ms;
+      v[k] = decode2(reinterpret_cast<const uint8_t*>(a.v)[si]).x * rs;
+      v[k] *= v[k];
+    } else {
+      m[k] = reinterpret_cast<const float*>(a.m)[si];
+      v[k] = reinterpret_cast<const float*>(a.v)[si];
+    }
+    p[k] = a.master ? a.master[si] : load_as_f32(t.param, t.dtype, i);
+  }
+  float ma = 0.f, ra = 0.f;
+  #pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint64_t i = b + lane + 32 * k, si = t.state + i;
+    update(s, keep, g[k], m[k], v[k], p[k], r[k]);
+    if (i >= end) continue;
+    if (a.master) a.master[si] = p[k];
+    store_from_f32(t.param, t.dtype, i, p[k]);
+    if constexpr (FP8) {
+      ma = fmaxf(ma, fabsf(m[k]));
+      ra = fmaxf(ra, r[k]);
+    } else {
+      reinterpret_cast<float*>(a.m)[si] = m[k];
+      reinterpret_cast<float*>(a.v)[si] = v[k];
+    }
+  }
+  if constexpr (FP8) {
+    ms = block_scale(warp_max(ma));
+    rs = block_scale(warp_max(ra));
+    const float mi = __frcp_rn(ms), ri = __frcp_rn(rs);
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t i = b + lane + 32 * k, si = t.state + i;
+      if (i >= end) continue;
+      reinterpret_cast<uint8_t*>(a.m)[si] = __nv_cvt_float_to_fp8(m[k] * mi, __NV_SATFINITE, __NV_E4M3);
+      reinterpret_cast<uint8_t*>(a.v)[si] = __nv_cvt_float_to_fp8(root_code(r[k], ri), __NV_SATFINITE, __NV_E4M3);
+    }
+    if (lane == 0) {
+      a.m_scale[blk] = ms;
+      a.v_scale[blk] = rs;
+    }
+  }
+}
+
+template <bool FP8, typename P, typename G>
+__device__ __forceinline__ void step_chunk(const AdamArgs& a, const StepScalars& s, float keep, const AdamTensor& t, uint64_t grad,
+                                           uint64_t begin, uint64_t end) {
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  P* param = reinterpret_cast<P*>(t.param);
+  const G* gp = reinterpret_cast<const G*>(grad);
+  const bool aligned = ((t.param % (8 * sizeof(P))) | (grad % (8 * sizeof(G)))) == 0;
+  for (uint64_t i = begin + warp * 256; i < end; i += kAdamTile) {
+    if (aligned && i + 256 <= end) {
+      const uint64_t j = i + lane * 8;
+      step_vector<FP8>(a, s, keep, param + j, gp + j, t.state + j);
+    } else {
+      const uint32_t gtype = sizeof(G) == 4 ? (uint32_t)DT_F32 : t.dtype;
+      step_block<FP8>(a, s, keep, t, grad, gtype, i, end);
+      if (i + kStateBlock < end) step_block<FP8>(a, s, keep, t, grad, gtype, i + kStateBlock, end);
+    }
+  }
+}
+
 template <bool FP8, int N>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const AdamArgs a, const __grid_constant__ Grads<N> g) {
-  __shared__ StepScalars s;
-  __shared__ bool skip;
+  __shared__ StepScalars shared;
+  __shared__ double red[kWarps];
+  double sum_sq = 0.0;
+  if (a.partial) {
+    for (uint32_t i = threadIdx.x; i < a.n_partial; i += kThreads) sum_sq += a.partial[i];
+    sum_sq = cta_sum(sum_sq, red);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && g.first_tensor == 0) *a.norm = (float)sqrt(sum_sq);
+    if (!(sum_sq <= kMaxDouble)) return;              // a step on gradients that are not finite is not taken
+  }
   if (threadIdx.x == 0) {
     const double lr = !a.lr_ptr ? a.lr : a.lr_f64 ? *reinterpret_cast<const double*>(a.lr_ptr) : (double)*reinterpret_cast<const float*>(a.lr_ptr);
     const double c1 = 1.0 - a.clock->b1t * a.beta1, c2 = 1.0 - a.clock->b2t * a.beta2;
-    double coef = 1.0;
-    skip = false;
-    if (a.sum_sq) {
-      const double norm = sqrt(*a.sum_sq);
-      coef = fmin(1.0, a.max_norm / (norm + 1e-6));
-      skip = !(norm <= 1.7976931348623157e308);       // a step on gradients that are not finite is not taken
-      if (blockIdx.x == 0 && g.first_tensor == 0) *a.norm = (float)norm;
-    }
-    s = StepScalars{(float)a.beta1, (float)(1.0 - a.beta1), (float)a.beta2, (float)(1.0 - a.beta2), (float)(lr / c1),
-                    (float)(1.0 / c2), (float)a.eps, (float)coef, lr};
+    const double coef = a.partial ? fmin(1.0, a.max_norm / (sqrt(sum_sq) + 1e-6)) : 1.0;
+    shared = StepScalars{(float)a.beta1, (float)(1.0 - a.beta1), (float)a.beta2, (float)(1.0 - a.beta2), (float)(lr / c1),
+                         (float)sqrt(1.0 / c2), (float)a.eps, (float)coef, (float)lr};
   }
   __syncthreads();
-  if (skip) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const StepScalars s = shared;
   for (uint32_t c = blockIdx.x; c < g.n_chunks; c += gridDim.x) {
     const AdamChunk ch = a.chunks[g.first_chunk + c];
-    const AdamTensor t = a.tensors[ch.tensor];
-    const uint64_t gp = g.p[ch.tensor - g.first_tensor];
+    const uint64_t gp = g.p[ch.tensor - g.first_tensor], grad = gp & ~1ull;
     if (gp == 0) continue;
-    const uint32_t gtype = gp & 1 ? (uint32_t)DT_F32 : t.dtype;
-    const float keep = (float)(1.0 - s.lr * t.weight_decay);
-    const uint64_t begin = (uint64_t)ch.chunk * kAdamChunk;
-    const uint64_t end = begin + kAdamChunk < t.numel ? begin + kAdamChunk : t.numel;
-    for (uint64_t b = begin + warp * kStateBlock; b < end; b += kThreads / 32 * kStateBlock) {
-      const uint64_t blk = (t.state + b) / kStateBlock;
-      float m[4], r[4], ma = 0.f, ra = 0.f;
-      #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint64_t i = b + lane + 32 * k, si = t.state + i;
-        m[k] = r[k] = 0.f;
-        if (i >= end) continue;
-        const float grad = load_as_f32(gp & ~1ull, gtype, i) * s.coef;
-        float m0, v0;
-        if constexpr (FP8) {
-          m0 = e4m3_to_f32(reinterpret_cast<const uint8_t*>(a.m)[si]) * a.m_scale[blk];
-          const float r0 = e4m3_to_f32(reinterpret_cast<const uint8_t*>(a.v)[si]) * a.v_scale[blk];
-          v0 = r0 * r0;
-        } else {
-          m0 = reinterpret_cast<const float*>(a.m)[si];
-          v0 = reinterpret_cast<const float*>(a.v)[si];
-        }
-        m[k] = s.b1 * m0 + s.om_b1 * grad;
-        const float v = s.b2 * v0 + s.om_b2 * grad * grad;
-        float p = a.master ? a.master[si] : load_as_f32(t.param, t.dtype, i);
-        p = p * keep - s.step_size * (m[k] / (sqrtf(v * s.inv_c2) + s.eps));
-        if (a.master) a.master[si] = p;
-        store_from_f32(t.param, t.dtype, i, p);
-        if constexpr (FP8) {
-          r[k] = sqrtf(v);
-          ma = fmaxf(ma, fabsf(m[k]));
-          ra = fmaxf(ra, r[k]);
-        } else {
-          reinterpret_cast<float*>(a.m)[si] = m[k];
-          reinterpret_cast<float*>(a.v)[si] = v;
-        }
-      }
-      if constexpr (FP8) {
-        const float ms = block_scale(warp_max(ma)), rs = block_scale(warp_max(ra));
-        const float mi = __frcp_rn(ms), ri = __frcp_rn(rs);
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t i = b + lane + 32 * k, si = t.state + i;
-          if (i >= end) continue;
-          reinterpret_cast<uint8_t*>(a.m)[si] = __nv_cvt_float_to_fp8(m[k] * mi, __NV_SATFINITE, __NV_E4M3);
-          uint8_t q = __nv_cvt_float_to_fp8(r[k] * ri, __NV_SATFINITE, __NV_E4M3);
-          if (r[k] > 0.f && q == 0) q = 1;
-          reinterpret_cast<uint8_t*>(a.v)[si] = q;
-        }
-        __syncwarp();       // every lane has read the old scales
-        if (lane == 0) {
-          a.m_scale[blk] = ms;
-          a.v_scale[blk] = rs;
-        }
-      }
-    }
+    const AdamTensor t = a.tensors[ch.tensor];
+    const float keep = (float)(1.0 - (double)s.lr * t.weight_decay);
+    const uint64_t begin = (uint64_t)ch.chunk * a.chunk, end = begin + a.chunk < t.numel ? begin + a.chunk : t.numel;
+    if (t.dtype == DT_F32) step_chunk<FP8, float, float>(a, s, keep, t, grad, begin, end);
+    else if (t.dtype == DT_BF16 && (gp & 1)) step_chunk<FP8, __nv_bfloat16, float>(a, s, keep, t, grad, begin, end);
+    else if (t.dtype == DT_BF16) step_chunk<FP8, __nv_bfloat16, __nv_bfloat16>(a, s, keep, t, grad, begin, end);
+    else if (gp & 1) step_chunk<FP8, __half, float>(a, s, keep, t, grad, begin, end);
+    else step_chunk<FP8, __half, __half>(a, s, keep, t, grad, begin, end);
   }
   // the last CTA of a step's last launch advances the clock; all others have read it by then
-  if (!g.last) return;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  if (g.last && threadIdx.x == 0) {
     __threadfence();
     if (atomicAdd(&a.clock->done, 1u) == gridDim.x - 1) {
       a.clock->done = 0;
@@ -157,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const AdamArgs a, const
 template <bool FP8, int N>
 cudaError_t adamw_launch_n(const AdamArgs& a, const uint64_t* grads, const uint32_t* chunk_start, uint32_t first, uint32_t n,
                            int sms, cudaStream_t stream) {
-  Grads<N> g{};
+  Grads<N> g;
   for (uint32_t i = 0; i < n; ++i) g.p[i] = grads[first + i];
   g.first_tensor = first;
   g.first_chunk = chunk_start[first];
@@ -182,27 +307,52 @@ cudaError_t adamw_launch(const AdamArgs& a, const uint64_t* grads, const uint32_
   return cudaSuccess;
 }
 
-// -- sum of squares -----------------------------------------------------------------------------
+// -- sum of squares -------------------------------------------------------------------------------
 template <int N>
 struct NormTable {
   NormTensor t[N];
   uint32_t n, n_chunks;
 };
 
-__device__ __forceinline__ double cta_sum(double v, double* red) {
-  #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int i = 0; i < kThreads / 32; ++i) v += red[i];
-  return v;
+// Elements [begin, end) counted from the 32-byte boundary at or below the tensor's start, of which
+// [mis, mis + numel) are the tensor's.  Each thread adds at most 64 squares in 32 bits.
+template <typename T>
+__device__ __forceinline__ float chunk_squares(const NormTensor& t, uint64_t begin) {
+  constexpr int V = kVecN<T>, kDepth = 4;
+  const T* x = reinterpret_cast<const T*>(t.ptr);
+  const uint32_t mis = (uint32_t)(t.ptr & 31) / sizeof(T);
+  const uint64_t end = t.numel + mis;
+  float sum = 0.f;
+  F2 acc{0.f, 0.f};
+  if (begin >= mis && begin + kNormChunk <= end) {
+    const T* p = x + (begin - mis) + threadIdx.x * V;
+    #pragma unroll
+    for (uint32_t k = 0; k < kNormChunk; k += kDepth * kThreads * V) {
+      Vec32 raw[kDepth];
+      #pragma unroll
+      for (int u = 0; u < kDepth; ++u) raw[u] = load32(p + k + u * kThreads * V);
+      #pragma unroll
+      for (int u = 0; u < kDepth; ++u) {
+        F2 v[V / 2];
+        unpack<T>(raw[u], v);
+        #pragma unroll
+        for (int i = 0; i < V / 2; ++i) acc = fma2(v[i], v[i], acc);
+      }
+    }
+    sum = acc.x + acc.y;
+  } else {
+    for (uint64_t i = begin + threadIdx.x; i < begin + kNormChunk && i < end; i += kThreads)
+      if (i >= mis) {
+        const float f = to_f32(x[i - mis]);
+        sum += f * f;
+      }
+  }
+  return sum;
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads) sum_sq_kernel(const __grid_constant__ NormTable<N> tab, double* partial) {
-  __shared__ double red[kThreads / 32];
+__global__ void __launch_bounds__(kThreads) partial_sums_kernel(const __grid_constant__ NormTable<N> tab, double* partial) {
+  __shared__ double red[kWarps];
   double acc = 0.0;
   for (uint32_t c = blockIdx.x; c < tab.n_chunks; c += gridDim.x) {
     uint32_t lo = 0, hi = tab.n;                  // the tensor whose chunks hold c
@@ -212,20 +362,15 @@ __global__ void __launch_bounds__(kThreads) sum_sq_kernel(const __grid_constant_
     }
     const NormTensor& t = tab.t[lo];
     const uint64_t begin = (uint64_t)(c - t.first_chunk) * kNormChunk;
-    const uint64_t end = begin + kNormChunk < t.numel ? begin + kNormChunk : t.numel;
-    float s = 0.f;                                // at most 64 squares; sums of those in 64 bits
-    for (uint64_t i = begin + threadIdx.x; i < end; i += kThreads) {
-      const float x = load_as_f32(t.ptr, t.dtype, i);
-      s += x * x;
-    }
-    acc += s;
+    acc += t.dtype == DT_F32 ? chunk_squares<float>(t, begin)
+           : t.dtype == DT_BF16 ? chunk_squares<__nv_bfloat16>(t, begin) : chunk_squares<__half>(t, begin);
   }
   acc = cta_sum(acc, red);
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
-__global__ void __launch_bounds__(kThreads) sum_sq_final_kernel(const double* partial, uint32_t n, double* sum_sq, float* norm) {
-  __shared__ double red[kThreads / 32];
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double* partial, uint32_t n, double* sum_sq, float* norm) {
+  __shared__ double red[kWarps];
   double acc = 0.0;
   for (uint32_t i = threadIdx.x; i < n; i += kThreads) acc += partial[i];
   acc = cta_sum(acc, red);
@@ -235,24 +380,25 @@ __global__ void __launch_bounds__(kThreads) sum_sq_final_kernel(const double* pa
   }
 }
 
-uint32_t norm_grid(uint32_t n_chunks, int sms) {
-  const uint32_t cap = (uint32_t)sms * 8u;
-  return n_chunks < cap ? n_chunks : cap;
+constexpr uint32_t kNormCtas = 4;         // per SM
+
+uint32_t chunks_of(const NormTensor& t) {
+  const uint64_t mis = (t.ptr & 31) / dtype_bytes(t.dtype);
+  return (uint32_t)((t.numel + mis + kNormChunk - 1) / kNormChunk);
 }
 
-uint32_t chunks_of(const NormTensor& t) { return (uint32_t)((t.numel + kNormChunk - 1) / kNormChunk); }
-
 template <int N>
-uint32_t sum_sq_launch_n(NormTensor* t, uint32_t n, double* partial, int sms, cudaStream_t stream) {
-  NormTable<N> tab{};
+uint32_t partial_sums_launch(NormTensor* t, uint32_t n, double* partial, int sms, cudaStream_t stream) {
+  NormTable<N> tab;
+  tab.n_chunks = 0;
   for (uint32_t i = 0; i < n; ++i) {
     t[i].first_chunk = tab.n_chunks;
     tab.n_chunks += chunks_of(t[i]);
     tab.t[i] = t[i];
   }
   tab.n = n;
-  const uint32_t grid = norm_grid(tab.n_chunks, sms);
-  if (grid) sum_sq_kernel<N><<<grid, kThreads, 0, stream>>>(tab, partial);
+  const uint32_t cap = (uint32_t)sms * kNormCtas, grid = tab.n_chunks < cap ? tab.n_chunks : cap;
+  if (grid) partial_sums_kernel<N><<<grid, kThreads, 0, stream>>>(tab, partial);
   return grid;
 }
 
@@ -262,21 +408,24 @@ cudaError_t launch_adamw(const AdamArgs& a, const uint64_t* grads, const uint32_
   return a.m_scale ? adamw_launch<true>(a, grads, chunk_start, sms, stream) : adamw_launch<false>(a, grads, chunk_start, sms, stream);
 }
 
-uint64_t sum_sq_scratch(const NormTensor* t, uint32_t n, int sms) {
-  const uint64_t launches = (n + kNormTensorsPerLaunch - 1) / kNormTensorsPerLaunch;
-  return launches * (uint64_t)sms * 8u + 1;
+uint64_t partial_sums_size(uint32_t n, int sms) {
+  return (uint64_t)((n + kNormTensorsPerLaunch - 1) / kNormTensorsPerLaunch) * (uint64_t)sms * kNormCtas;
 }
 
-cudaError_t launch_sum_sq(NormTensor* t, uint32_t n, double* scratch, double* sum_sq, float* norm, int sms, cudaStream_t stream) {
-  uint32_t used = 0;
+cudaError_t launch_partial_sums(NormTensor* t, uint32_t n, double* partial, uint32_t* n_partial, int sms, cudaStream_t stream) {
+  *n_partial = 0;
   for (uint32_t first = 0; first < n; first += kNormTensorsPerLaunch) {
     const uint32_t k = n - first < kNormTensorsPerLaunch ? n - first : kNormTensorsPerLaunch;
-    used += k <= 128 ? sum_sq_launch_n<128>(t + first, k, scratch + used, sms, stream)
-                     : sum_sq_launch_n<kNormTensorsPerLaunch>(t + first, k, scratch + used, sms, stream);
+    *n_partial += k <= 128 ? partial_sums_launch<128>(t + first, k, partial + *n_partial, sms, stream)
+                           : partial_sums_launch<kNormTensorsPerLaunch>(t + first, k, partial + *n_partial, sms, stream);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  sum_sq_final_kernel<<<1, kThreads, 0, stream>>>(scratch, used, sum_sq, norm);
+  return cudaSuccess;
+}
+
+cudaError_t launch_norm(const double* partial, uint32_t n_partial, double* sum_sq, float* norm, cudaStream_t stream) {
+  norm_kernel<<<1, kThreads, 0, stream>>>(partial, n_partial, sum_sq, norm);
   return cudaGetLastError();
 }
 

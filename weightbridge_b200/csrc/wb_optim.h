@@ -9,8 +9,8 @@
 namespace wb {
 
 constexpr uint32_t kStateBlock = 128;     // elements that share a scale in the 8-bit states
-constexpr uint32_t kAdamChunk = 8192;     // elements of one work item of the step
-constexpr uint32_t kNormChunk = 16384;
+constexpr uint32_t kAdamTile = 2048;      // elements that a CTA of the step takes at once; a work item is a multiple
+constexpr uint32_t kNormChunk = 16384;    // elements of one work item of the norm
 
 // One parameter tensor (resident on the GPU).
 struct alignas(16) AdamTensor {
@@ -24,7 +24,7 @@ static_assert(sizeof(AdamTensor) == 32, "AdamTensor layout");
 
 struct AdamChunk {
   uint32_t tensor;
-  uint32_t chunk;          // elements [chunk * kAdamChunk, ...)
+  uint32_t chunk;          // elements [chunk * AdamArgs::chunk, ...)
 };
 
 // The device's own record of the steps taken, so that a captured step can be replayed.
@@ -40,6 +40,7 @@ struct AdamArgs {
   const AdamTensor* tensors;
   const AdamChunk* chunks;
   uint32_t n_tensors;
+  uint32_t chunk;          // elements of a work item
   float* master;           // flat, or null
   void* m;                 // flat fp32, or e4m3
   void* v;                 // flat fp32 second moment, or e4m3 of its root
@@ -51,9 +52,10 @@ struct AdamArgs {
   const void* lr_ptr;      // device scalar instead of lr, or null
   int lr_f64;
   double eps;
-  const double* sum_sq;    // squared gradient norm, or null: no clipping
+  const double* partial;   // the squared gradient norm is the sum of these; null: no clipping
+  uint32_t n_partial;
   double max_norm;
-  float* norm;             // receives the norm (with sum_sq)
+  float* norm;             // receives the norm (with partial)
 };
 
 // Gradients travel as launch arguments: their addresses change from step to step, and arguments
@@ -73,9 +75,11 @@ struct NormTensor {
 static_assert(sizeof(NormTensor) == 24, "NormTensor layout");
 constexpr uint32_t kNormTensorsPerLaunch = 1300;
 
-// Doubles of scratch that launch_sum_sq needs.
-uint64_t sum_sq_scratch(const NormTensor* t, uint32_t n, int sms);
-// sum_sq[0] = sum of squares over all tensors (in a fixed order), norm[0] = its root.
-cudaError_t launch_sum_sq(NormTensor* t, uint32_t n, double* scratch, double* sum_sq, float* norm, int sms, cudaStream_t stream);
+// Partial sums of squares that launch_partial_sums writes over all tensors, at most.
+uint64_t partial_sums_size(uint32_t n, int sms);
+// Writes partial sums (a fixed split of the work, so the same bits every time); *n_partial of them.
+cudaError_t launch_partial_sums(NormTensor* t, uint32_t n, double* partial, uint32_t* n_partial, int sms, cudaStream_t stream);
+// sum_sq[0] = the sum of the partial sums, norm[0] = its root.
+cudaError_t launch_norm(const double* partial, uint32_t n_partial, double* sum_sq, float* norm, cudaStream_t stream);
 
 }  // namespace wb

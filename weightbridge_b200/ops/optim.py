@@ -93,10 +93,9 @@ class AdamW:
             return p.step(grads, number, on_device, None, 0.0)
         if not max_norm > 0.0:
             raise ValueError(f"AdamW.step: max_norm must be positive, not {max_norm}")
-        sum_sq = p.grad_sum_sq(grads)
+        sum_sq = None                           # the kernels' own, from these gradients
         if group is not None:
-            if sum_sq is None:                  # a rank without gradients still takes part in the reduction
-                sum_sq = torch.zeros((), dtype=torch.float64, device=p.exp_avg.device)
+            sum_sq = p.grad_sum_sq(grads)
             torch.distributed.all_reduce(sum_sq, group=group)
         return p.step(grads, number, on_device, sum_sq, float(max_norm))
 
