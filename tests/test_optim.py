@@ -100,11 +100,11 @@ def _step_and_check(params, grads, opt, lr=1e-2, max_norm=None, wd=0.1, no_decay
             scale = want_s.repeat_interleave(128)[:x.numel()]
             tiny = (x.abs() < scale * 2.0 ** -9) & (x.abs() > 0)
             half = x.abs() * 2.0 ** -4 + scale * 2.0 ** -10
-            if key == "rms_scale":      # a positive root keeps the smallest code; squares below 2^-149 are 0 in 32 bits
-                pos = x > 2.0 ** -74
+            if key == "rms_scale":      # a positive root keeps the smallest code; squares below 2^-126 may count as 0
+                pos = x > 2.0 ** -63
                 assert bool((got[pos] >= scale[pos] * 2.0 ** -9 * (1 - 1e-5)).all())
                 half = torch.where(tiny, scale * 2.0 ** -9, half)
-            least = 2.0 ** -74 if key == "rms_scale" else 1e-45     # roots of what 32 bits cannot hold
+            least = 2.0 ** -63 if key == "rms_scale" else 1e-45     # roots of what 32 bits do not hold as normal numbers
             bad = (got - x).abs() > half * 1.0001 + tol_x + least
             assert not bool(bad.any()), (n, key, int(bad.sum()))
             assert bool((got[x == 0] == 0).all())

@@ -302,9 +302,9 @@ struct AdamWProgram {
     }
     const c10::cuda::CUDAGuard guard(dev);
     sms = sm_count(dev.index());
-    // A work item: four tiles where the SMs still get eight items each, which reads a tensor's entry
-    // once for all four; one tile for small models, where it takes many CTAs to fill the GPU at all.
-    chunk = total >= (int64_t)sms * 8 * 4 * wb::kAdamTile ? 4 * wb::kAdamTile : wb::kAdamTile;
+    // A work item: two tiles where the SMs still get sixteen items each, which reads a tensor's entry
+    // once for both; one for smaller models, where it takes many CTAs to fill the GPU at all.
+    chunk = total >= (int64_t)sms * 16 * 2 * wb::kAdamTile ? 2 * wb::kAdamTile : wb::kAdamTile;
     for (const Tensor& p : params) {
       chunk_start.push_back((uint32_t)n_chunks);
       n_chunks += ((uint64_t)p.numel() + chunk - 1) / chunk;

@@ -55,181 +55,200 @@ struct Grads {
   uint32_t first_tensor, first_chunk, n_chunks, last;
 };
 
-__device__ __forceinline__ float root(float x) {          // relative error 2^-23
+// Hardware approximations with relative errors of 2^-23; numbers below 2^-126 count as 0.
+__device__ __forceinline__ float root(float x) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ F2 both(float x) { return {x, x}; }
 
-// One element: the new moments, the new value and r = sqrt(v).
-__device__ __forceinline__ void update(const StepScalars& s, float keep, float grad, float& m, float& v, float& p, float& r) {
-  const float g = grad * s.coef;
-  m = s.b1 * m + s.om_b1 * g;
-  v = s.b2 * v + s.om_b2 * g * g;
-  r = root(v);
-  p = p * keep - s.step_size * __fdividef(m, r * s.root_c2 + s.eps);
+// Two elements: the new moments, the new values and r = sqrt(v).
+__device__ __forceinline__ void update2(const StepScalars& s, float keep, F2 grad, F2& m, F2& v, F2& p, F2& r) {
+  const F2 g = mul2(grad, both(s.coef));
+  m = fma2(both(s.b1), m, mul2(both(s.om_b1), g));
+  v = fma2(both(s.b2), v, mul2(mul2(both(s.om_b2), g), g));
+  r = {root(v.x), root(v.y)};
+  const F2 d = fma2(r, both(s.root_c2), both(s.eps));
+  const F2 u = mul2(m, F2{reciprocal(d.x), reciprocal(d.y)});
+  p = fma2(both(-s.step_size), u, mul2(p, both(keep)));
 }
 
-__device__ __forceinline__ float2 decode2(uint32_t q) {
+__device__ __forceinline__ F2 decode2(uint32_t q) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q & 0xffffu), __NV_E4M3);
-  return __half22float2(__half2(h));
+  const float2 f = __half22float2(__half2(h));
+  return {f.x, f.y};
 }
 
-__device__ __forceinline__ void decode8(uint2 q, float scale, float (&x)[8]) {
-  const uint32_t w[4] = {q.x, q.x >> 16, q.y, q.y >> 16};
-  #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = decode2(w[i]);
-    x[2 * i] = f.x * scale;
-    x[2 * i + 1] = f.y * scale;
-  }
-}
+__device__ __forceinline__ uint32_t encode2(F2 x) { return __nv_cvt_float2_to_fp8x2(make_float2(x.x, x.y), __NV_SATFINITE, __NV_E4M3); }
 
-__device__ __forceinline__ uint2 encode8(const float (&x)[8]) {
-  uint32_t w[4];
-  #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-}
-
-// scale of a block; tiny blocks keep a normal scale, whose reciprocal is finite
+// Scale of a block, amax / 448, and 448 / amax, each with one correction step after the product
+// (the reciprocal of the rounded scale would round once more).  A block of tiny values keeps a
+// normal scale, whose reciprocal is finite; a block of zeros has scale 1.
 __device__ __forceinline__ float block_scale(float amax) {
-  return amax > 0.f ? fmaxf(__fdiv_rn(amax, kE4M3Max), 1.17549435e-38f) : 1.f;
+  constexpr float kInv = 1.f / kE4M3Max;
+  float q = amax * kInv;
+  q = fmaf(fmaf(-kE4M3Max, q, amax), kInv, q);
+  return amax > 0.f ? fmaxf(q, 1.17549435e-38f) : 1.f;
+}
+__device__ __forceinline__ float block_inverse(float amax) {
+  const float r = reciprocal(amax);
+  float q = kE4M3Max * r;
+  q = fmaf(fmaf(-amax, q, kE4M3Max), r, q);
+  return fminf(q, 8.507059173e37f);         // 2^126, also where the above is not a number (zero and tiny blocks)
 }
 
-// r / scale, where a positive r keeps at least the smallest code
-__device__ __forceinline__ float root_code(float r, float inv) { return fmaxf(r * inv, r > 0.f ? 0.001953125f : 0.f); }
+// r in units of the scale; a positive r keeps at least the smallest code
+__device__ __forceinline__ F2 root_codes(F2 r, float inv) {
+  const F2 q = mul2(r, both(inv));
+  return {fmaxf(q.x, r.x > 0.f ? 0.001953125f : 0.f), fmaxf(q.y, r.y > 0.f ? 0.001953125f : 0.f)};
+}
 
-// 256 elements from element i0 of the tensor on, eight a lane, all addresses aligned to eight
-// elements: 16 lanes hold a block of the 8-bit states.
+// E consecutive elements of the states of one lane, as pairs.  Slices of the flat buffers are
+// padded to whole blocks, so a lane may pass the tensor's end: there the states are and stay 0.
+template <bool FP8, int E>
+struct States {
+  F2 m[E / 2], v[E / 2];
+
+  __device__ __forceinline__ void load(const AdamArgs& a, uint64_t si) {
+    if constexpr (FP8) {
+      uint32_t mq[E / 4], vq[E / 4];
+      read_codes(reinterpret_cast<const uint8_t*>(a.m) + si, mq);
+      read_codes(reinterpret_cast<const uint8_t*>(a.v) + si, vq);
+      const F2 ms = both(a.m_scale[si / kStateBlock]), vs = both(a.v_scale[si / kStateBlock]);
+      #pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        m[i] = mul2(decode2(i & 1 ? mq[i / 2] >> 16 : mq[i / 2]), ms);
+        const F2 r = mul2(decode2(i & 1 ? vq[i / 2] >> 16 : vq[i / 2]), vs);
+        v[i] = mul2(r, r);
+      }
+    } else {
+      load_pairs<E>(reinterpret_cast<const float*>(a.m) + si, m);
+      load_pairs<E>(reinterpret_cast<const float*>(a.v) + si, v);
+    }
+  }
+
+  // r: the roots of v
+  __device__ __forceinline__ void store(const AdamArgs& a, uint64_t si, const F2 (&r)[E / 2]) {
+    if constexpr (FP8) {
+      constexpr int kLanes = kStateBlock / E;            // lanes that share a block
+      float ma = 0.f, ra = 0.f;
+      #pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        ma = fmaxf(ma, fmaxf(fabsf(m[i].x), fabsf(m[i].y)));
+        ra = fmaxf(ra, fmaxf(r[i].x, r[i].y));
+      }
+      #pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+        ma = fmaxf(ma, __shfl_xor_sync(kFullWarp, ma, o));
+        ra = fmaxf(ra, __shfl_xor_sync(kFullWarp, ra, o));
+      }
+      const float mi = block_inverse(ma), ri = block_inverse(ra);
+      uint32_t mq[E / 4], vq[E / 4];
+      #pragma unroll
+      for (int i = 0; i < E / 4; ++i) {
+        mq[i] = encode2(mul2(m[2 * i], both(mi))) | encode2(mul2(m[2 * i + 1], both(mi))) << 16;
+        vq[i] = encode2(root_codes(r[2 * i], ri)) | encode2(root_codes(r[2 * i + 1], ri)) << 16;
+      }
+      write_codes(reinterpret_cast<uint8_t*>(a.m) + si, mq);
+      write_codes(reinterpret_cast<uint8_t*>(a.v) + si, vq);
+      if ((threadIdx.x & (kLanes - 1)) == 0) {           // the lanes' shuffles came after their loads of the old scales
+        a.m_scale[si / kStateBlock] = block_scale(ma);
+        a.v_scale[si / kStateBlock] = block_scale(ra);
+      }
+    } else {
+      store_pairs<E>(reinterpret_cast<float*>(a.m) + si, m);
+      store_pairs<E>(reinterpret_cast<float*>(a.v) + si, v);
+    }
+  }
+
+ private:
+  __device__ __forceinline__ static void read_codes(const uint8_t* p, uint32_t (&q)[E / 4]) {
+    if constexpr (E == 16) {
+      const uint4 w = load16(p);
+      q[0] = w.x, q[1] = w.y, q[2] = w.z, q[3] = w.w;
+    } else {
+      static_assert(E == 4);
+      q[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+  }
+  __device__ __forceinline__ static void write_codes(uint8_t* p, const uint32_t (&q)[E / 4]) {
+    if constexpr (E == 16) store16(p, make_uint4(q[0], q[1], q[2], q[3]));
+    else *reinterpret_cast<uint32_t*>(p) = q[0];
+  }
+};
+
+// E elements a lane with vectors, all addresses aligned to them.  Eight for fp32 states (64 bytes
+// of them in flight a lane), sixteen for 8-bit ones (16-byte loads of codes, eight lanes a block).
+template <bool FP8> constexpr int kLaneElems = FP8 ? 16 : 8;
+
 template <bool FP8, typename P, typename G>
 __device__ __forceinline__ void step_vector(const AdamArgs& a, const StepScalars& s, float keep, P* param, const G* grad, uint64_t si) {
-  float g[8], m[8], v[8], p[8], r[8];
-  load_eight(grad, g);
-  const uint64_t blk = si / kStateBlock;
-  float ms = 0.f, rs = 0.f;
-  uint2 mq, rq;
-  if constexpr (FP8) {
-    mq = load8(reinterpret_cast<const uint8_t*>(a.m) + si);
-    rq = load8(reinterpret_cast<const uint8_t*>(a.v) + si);
-    ms = a.m_scale[blk];
-    rs = a.v_scale[blk];
-  } else {
-    load_eight(reinterpret_cast<const float*>(a.m) + si, m);
-    load_eight(reinterpret_cast<const float*>(a.v) + si, v);
-  }
-  if (a.master) load_eight(a.master + si, p);
-  else load_eight(param, p);
-  if constexpr (FP8) {
-    decode8(mq, ms, m);
-    decode8(rq, rs, v);
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= v[i];
-  }
+  constexpr int E = kLaneElems<FP8>;
+  F2 g[E / 2], p[E / 2], r[E / 2];
+  States<FP8, E> st;
+  load_pairs<E>(grad, g);
+  if (a.master) load_pairs<E>(a.master + si, p);
+  else load_pairs<E>(param, p);
+  st.load(a, si);
   #pragma unroll
-  for (int i = 0; i < 8; ++i) update(s, keep, g[i], m[i], v[i], p[i], r[i]);
-  if (a.master) store_eight(a.master + si, p);
-  store_eight(param, p);
-  if constexpr (FP8) {
-    float ma = 0.f, ra = 0.f;
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) ma = fmaxf(ma, fabsf(m[i])), ra = fmaxf(ra, r[i]);
-    #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      ma = fmaxf(ma, __shfl_xor_sync(kFullWarp, ma, o));
-      ra = fmaxf(ra, __shfl_xor_sync(kFullWarp, ra, o));
-    }
-    ms = block_scale(ma);
-    rs = block_scale(ra);
-    const float mi = __frcp_rn(ms), ri = __frcp_rn(rs);
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] *= mi, r[i] = root_code(r[i], ri);
-    store8(reinterpret_cast<uint8_t*>(a.m) + si, encode8(m));
-    store8(reinterpret_cast<uint8_t*>(a.v) + si, encode8(r));
-    if ((threadIdx.x & 15) == 0) {        // the lanes' shuffles came after their loads of the old scales
-      a.m_scale[blk] = ms;
-      a.v_scale[blk] = rs;
-    }
-  } else {
-    store_eight(reinterpret_cast<float*>(a.m) + si, m);
-    store_eight(reinterpret_cast<float*>(a.v) + si, v);
-  }
+  for (int i = 0; i < E / 2; ++i) update2(s, keep, g[i], st.m[i], st.v[i], p[i], r[i]);
+  if (a.master) store_pairs<E>(a.master + si, p);
+  store_pairs<E>(param, p);
+  st.store(a, si, r);
 }
 
-// One block of 128 elements, or what is left of the tensor: single elements side by side, four a
-// lane, for tensors at odd addresses and for their ends.
-template <bool FP8>
-__device__ __forceinline__ void step_block(const AdamArgs& a, const StepScalars& s, float keep, const AdamTensor& t, uint64_t grad,
-                                           uint32_t gtype, uint64_t b, uint64_t end) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t blk = (t.state + b) / kStateBlock;
-  float m[4], v[4], r[4], p[4], g[4], ms = 0.f, rs = 0.f;
-  if constexpr (FP8) ms = a.m_scale[blk], rs = a.v_scale[blk];
+// A block of 128 elements, four a lane: parameters and gradients one by one, for tensors at odd
+// addresses (FULL) and for the ends of tensors.  The states keep their vectors.
+template <bool FP8, bool FULL, typename P, typename G>
+__device__ __forceinline__ void step_block(const AdamArgs& a, const StepScalars& s, float keep, P* param, const G* grad, uint64_t si, uint32_t left) {
+  float g[4], p[4];
+  States<FP8, 4> st;
   #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint64_t i = b + lane + 32 * k, si = t.state + i;
-    m[k] = v[k] = g[k] = p[k] = 0.f;
-    if (i >= end) continue;
-    g[k] = load_as_f32(grad, gtype, i);
-    if constexpr (FP8) {
-      m[k] = decode2(reinterpret_cast<const uint8_t*>(a.m)[si]).x * ms;
-      v[k] = decode2(reinterpret_cast<const uint8_t*>(a.v)[si]).x * rs;
-      v[k] *= v[k];
-    } else {
-      m[k] = reinterpret_cast<const float*>(a.m)[si];
-      v[k] = reinterpret_cast<const float*>(a.v)[si];
-    }
-    p[k] = a.master ? a.master[si] : load_as_f32(t.param, t.dtype, i);
-  }
-  float ma = 0.f, ra = 0.f;
-  #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint64_t i = b + lane + 32 * k, si = t.state + i;
-    update(s, keep, g[k], m[k], v[k], p[k], r[k]);
-    if (i >= end) continue;
-    if (a.master) a.master[si] = p[k];
-    store_from_f32(t.param, t.dtype, i, p[k]);
-    if constexpr (FP8) {
-      ma = fmaxf(ma, fabsf(m[k]));
-      ra = fmaxf(ra, r[k]);
-    } else {
-      reinterpret_cast<float*>(a.m)[si] = m[k];
-      reinterpret_cast<float*>(a.v)[si] = v[k];
-    }
-  }
-  if constexpr (FP8) {
-    ms = block_scale(warp_max(ma));
-    rs = block_scale(warp_max(ra));
-    const float mi = __frcp_rn(ms), ri = __frcp_rn(rs);
+  for (int k = 0; k < 4; ++k) g[k] = FULL || k < left ? to_f32(grad[k]) : 0.f;
+  if (a.master) {
+    F2 w[2];
+    load_pairs<4>(a.master + si, w);
+    p[0] = w[0].x, p[1] = w[0].y, p[2] = w[1].x, p[3] = w[1].y;
+  } else {
     #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint64_t i = b + lane + 32 * k, si = t.state + i;
-      if (i >= end) continue;
-      reinterpret_cast<uint8_t*>(a.m)[si] = __nv_cvt_float_to_fp8(m[k] * mi, __NV_SATFINITE, __NV_E4M3);
-      reinterpret_cast<uint8_t*>(a.v)[si] = __nv_cvt_float_to_fp8(root_code(r[k], ri), __NV_SATFINITE, __NV_E4M3);
-    }
-    if (lane == 0) {
-      a.m_scale[blk] = ms;
-      a.v_scale[blk] = rs;
-    }
+    for (int k = 0; k < 4; ++k) p[k] = FULL || k < left ? to_f32(param[k]) : 0.f;
   }
+  st.load(a, si);
+  F2 w[2] = {{p[0], p[1]}, {p[2], p[3]}}, r[2];
+  update2(s, keep, {g[0], g[1]}, st.m[0], st.v[0], w[0], r[0]);
+  update2(s, keep, {g[2], g[3]}, st.m[1], st.v[1], w[1], r[1]);
+  if (a.master) store_pairs<4>(a.master + si, w);
+  p[0] = w[0].x, p[1] = w[0].y, p[2] = w[1].x, p[3] = w[1].y;
+  #pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (FULL || k < left) param[k] = from_f32<P>(p[k]);
+  st.store(a, si, r);
 }
 
 template <bool FP8, typename P, typename G>
 __device__ __forceinline__ void step_chunk(const AdamArgs& a, const StepScalars& s, float keep, const AdamTensor& t, uint64_t grad,
                                            uint64_t begin, uint64_t end) {
+  constexpr uint32_t kSpan = 32 * kLaneElems<FP8>;        // elements of a warp's step
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   P* param = reinterpret_cast<P*>(t.param);
   const G* gp = reinterpret_cast<const G*>(grad);
-  const bool aligned = ((t.param % (8 * sizeof(P))) | (grad % (8 * sizeof(G)))) == 0;
-  for (uint64_t i = begin + warp * 256; i < end; i += kAdamTile) {
-    if (aligned && i + 256 <= end) {
-      const uint64_t j = i + lane * 8;
+  const bool aligned = ((t.param | grad) & 31) == 0;
+  for (uint64_t i = begin + warp * kSpan; i < end; i += kWarps * kSpan) {
+    if (aligned && i + kSpan <= end) {
+      const uint64_t j = i + lane * kLaneElems<FP8>;
       step_vector<FP8>(a, s, keep, param + j, gp + j, t.state + j);
     } else {
-      const uint32_t gtype = sizeof(G) == 4 ? (uint32_t)DT_F32 : t.dtype;
-      step_block<FP8>(a, s, keep, t, grad, gtype, i, end);
-      if (i + kStateBlock < end) step_block<FP8>(a, s, keep, t, grad, gtype, i + kStateBlock, end);
+      for (uint64_t b = i; b < i + kSpan && b < end; b += kStateBlock) {
+        const uint64_t j = b + lane * 4;
+        if (b + kStateBlock <= end) step_block<FP8, true>(a, s, keep, param + j, gp + j, t.state + j, 4);
+        else step_block<FP8, false>(a, s, keep, param + j, gp + j, t.state + j, j < end ? (uint32_t)(end - j) : 0u);
+      }
     }
   }
 }

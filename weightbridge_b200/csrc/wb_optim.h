@@ -9,7 +9,7 @@
 namespace wb {
 
 constexpr uint32_t kStateBlock = 128;     // elements that share a scale in the 8-bit states
-constexpr uint32_t kAdamTile = 2048;      // elements that a CTA of the step takes at once; a work item is a multiple
+constexpr uint32_t kAdamTile = 4096;      // a work item of the step is a multiple of this; a CTA takes 2048 or 4096 at once
 constexpr uint32_t kNormChunk = 16384;    // elements of one work item of the norm
 
 // One parameter tensor (resident on the GPU).

@@ -33,15 +33,6 @@ __device__ __forceinline__ uint4 load16(const void* p) {
 __device__ __forceinline__ void store16(void* p, uint4 v) {
   asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ uint2 load8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void store8(void* p, uint2 v) {
-  asm volatile("st.global.v2.b32 [%0], {%1,%2};" ::"l"(p), "r"(v.x), "r"(v.y) : "memory");
-}
-
 template <typename T> constexpr int kVecN = 32 / (int)sizeof(T);
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -122,34 +113,49 @@ __device__ __forceinline__ Vec32 pack(const F2 (&x)[kVecN<T> / 2]) {
   return v;
 }
 
-// Eight consecutive elements as fp32: 16 or 32 bytes.
-template <typename T>
-__device__ __forceinline__ void load_eight(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const Vec32 v = load32(p);
+// E consecutive elements as pairs of fp32, in the widest vectors that they fill; p is aligned to
+// them, or to 32 bytes where they are longer.
+template <int E, typename T>
+__device__ __forceinline__ void load_pairs(const T* p, F2 (&x)[E / 2]) {
+  constexpr int kBytes = E * (int)sizeof(T);
+  if constexpr (kBytes >= 32) {
     #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v.w[i]);
+    for (int k = 0; k < kBytes / 32; ++k) {
+      F2 part[kVecN<T> / 2];
+      unpack<T>(load32(p + k * kVecN<T>), part);
+      #pragma unroll
+      for (int i = 0; i < kVecN<T> / 2; ++i) x[k * (kVecN<T> / 2) + i] = part[i];
+    }
   } else {
+    static_assert(kBytes == 16);
     const uint4 v = load16(p);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const F2 f = unpack2(w[i], T{});
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
+    for (int i = 0; i < E / 2; ++i) {
+      if constexpr (sizeof(T) == 4) x[i] = {__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])};
+      else x[i] = unpack2(w[i], T{});
     }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_eight(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    Vec32 v;
+template <int E, typename T>
+__device__ __forceinline__ void store_pairs(T* p, const F2 (&x)[E / 2]) {
+  constexpr int kBytes = E * (int)sizeof(T);
+  if constexpr (kBytes >= 32) {
     #pragma unroll
-    for (int i = 0; i < 8; ++i) v.w[i] = __float_as_uint(x[i]);
-    store32(p, v);
+    for (int k = 0; k < kBytes / 32; ++k) {
+      F2 part[kVecN<T> / 2];
+      #pragma unroll
+      for (int i = 0; i < kVecN<T> / 2; ++i) part[i] = x[k * (kVecN<T> / 2) + i];
+      store32(p + k * kVecN<T>, pack<T>(part));
+    }
   } else {
-    store16(p, make_uint4(pack2({x[0], x[1]}, T{}), pack2({x[2], x[3]}, T{}), pack2({x[4], x[5]}, T{}), pack2({x[6], x[7]}, T{})));
+    static_assert(kBytes == 16);
+    if constexpr (sizeof(T) == 4) {
+      store16(p, make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y)));
+    } else {
+      store16(p, make_uint4(pack2(x[0], T{}), pack2(x[1], T{}), pack2(x[2], T{}), pack2(x[3], T{})));
+    }
   }
 }
 
