@@ -302,9 +302,10 @@ struct AdamWProgram {
     }
     const c10::cuda::CUDAGuard guard(dev);
     sms = sm_count(dev.index());
-    // A work item: two tiles where the SMs still get sixteen items each, which reads a tensor's entry
-    // once for both; one for smaller models, where it takes many CTAs to fill the GPU at all.
-    chunk = total >= (int64_t)sms * 16 * 2 * wb::kAdamTile ? 2 * wb::kAdamTile : wb::kAdamTile;
+    // A work item: up to eight tiles, as long as every SM gets sixteen items.  A CTA reads a tensor's
+    // entry once per item and overlaps its loads within it; small models need the CTAs instead.
+    chunk = 8 * wb::kAdamTile;
+    while (chunk > wb::kAdamTile && total < (int64_t)sms * 16 * chunk) chunk /= 2;
     for (const Tensor& p : params) {
       chunk_start.push_back((uint32_t)n_chunks);
       n_chunks += ((uint64_t)p.numel() + chunk - 1) / chunk;

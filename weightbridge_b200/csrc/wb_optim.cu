@@ -49,6 +49,8 @@ __device__ __forceinline__ double cta_sum(double v, double* red) {
 // -- the step -------------------------------------------------------------------------------------
 struct StepScalars { float b1, om_b1, b2, om_b2, step_size, root_c2, eps, coef, lr; };
 
+template <bool FP8> constexpr int kAdamCtas = FP8 ? 2 : 4;       // CTAs an SM holds
+
 template <int N>
 struct Grads {
   uint64_t p[N];
@@ -109,27 +111,59 @@ __device__ __forceinline__ F2 root_codes(F2 r, float inv) {
   return {fmaxf(q.x, r.x > 0.f ? 0.001953125f : 0.f), fmaxf(q.y, r.y > 0.f ? 0.001953125f : 0.f)};
 }
 
-// E consecutive elements of the states of one lane, as pairs.  Slices of the flat buffers are
+// What one lane loads of the states of E consecutive elements, as it comes from memory.
+template <bool FP8, int E> struct RawStates;
+
+template <int E>
+struct RawStates<true, E> {
+  uint32_t m[E / 4], v[E / 4];
+  float ms, vs;
+  __device__ __forceinline__ void load(const AdamArgs& a, uint64_t si) {
+    read(reinterpret_cast<const uint8_t*>(a.m) + si, m);
+    read(reinterpret_cast<const uint8_t*>(a.v) + si, v);
+    ms = a.m_scale[si / kStateBlock];
+    vs = a.v_scale[si / kStateBlock];
+  }
+  __device__ __forceinline__ static void read(const uint8_t* p, uint32_t (&q)[E / 4]) {
+    if constexpr (E == 16) {
+      const uint4 w = load16(p);
+      q[0] = w.x, q[1] = w.y, q[2] = w.z, q[3] = w.w;
+    } else if constexpr (E == 8) {
+      const uint2 w = load8(p);
+      q[0] = w.x, q[1] = w.y;
+    } else {
+      static_assert(E == 4);
+      q[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+  }
+};
+
+template <int E>
+struct RawStates<false, E> {
+  F2 m[E / 2], v[E / 2];
+  __device__ __forceinline__ void load(const AdamArgs& a, uint64_t si) {
+    load_pairs<E>(reinterpret_cast<const float*>(a.m) + si, m);
+    load_pairs<E>(reinterpret_cast<const float*>(a.v) + si, v);
+  }
+};
+
+// The states of E consecutive elements of one lane, as pairs.  Slices of the flat buffers are
 // padded to whole blocks, so a lane may pass the tensor's end: there the states are and stay 0.
 template <bool FP8, int E>
 struct States {
   F2 m[E / 2], v[E / 2];
 
-  __device__ __forceinline__ void load(const AdamArgs& a, uint64_t si) {
-    if constexpr (FP8) {
-      uint32_t mq[E / 4], vq[E / 4];
-      read_codes(reinterpret_cast<const uint8_t*>(a.m) + si, mq);
-      read_codes(reinterpret_cast<const uint8_t*>(a.v) + si, vq);
-      const F2 ms = both(a.m_scale[si / kStateBlock]), vs = both(a.v_scale[si / kStateBlock]);
-      #pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        m[i] = mul2(decode2(i & 1 ? mq[i / 2] >> 16 : mq[i / 2]), ms);
-        const F2 r = mul2(decode2(i & 1 ? vq[i / 2] >> 16 : vq[i / 2]), vs);
+  __device__ __forceinline__ void decode(const RawStates<FP8, E>& raw) {
+    #pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      if constexpr (FP8) {
+        m[i] = mul2(decode2(i & 1 ? raw.m[i / 2] >> 16 : raw.m[i / 2]), both(raw.ms));
+        const F2 r = mul2(decode2(i & 1 ? raw.v[i / 2] >> 16 : raw.v[i / 2]), both(raw.vs));
         v[i] = mul2(r, r);
+      } else {
+        m[i] = raw.m[i];
+        v[i] = raw.v[i];
       }
-    } else {
-      load_pairs<E>(reinterpret_cast<const float*>(a.m) + si, m);
-      load_pairs<E>(reinterpret_cast<const float*>(a.v) + si, v);
     }
   }
 
@@ -168,93 +202,222 @@ struct States {
   }
 
  private:
-  __device__ __forceinline__ static void read_codes(const uint8_t* p, uint32_t (&q)[E / 4]) {
-    if constexpr (E == 16) {
-      const uint4 w = load16(p);
-      q[0] = w.x, q[1] = w.y, q[2] = w.z, q[3] = w.w;
-    } else {
-      static_assert(E == 4);
-      q[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-  }
   __device__ __forceinline__ static void write_codes(uint8_t* p, const uint32_t (&q)[E / 4]) {
     if constexpr (E == 16) store16(p, make_uint4(q[0], q[1], q[2], q[3]));
+    else if constexpr (E == 8) store8(p, make_uint2(q[0], q[1]));
     else *reinterpret_cast<uint32_t*>(p) = q[0];
   }
 };
 
-// E elements a lane with vectors, all addresses aligned to them.  Eight for fp32 states (64 bytes
-// of them in flight a lane), sixteen for 8-bit ones (16-byte loads of codes, eight lanes a block).
-template <bool FP8> constexpr int kLaneElems = FP8 ? 16 : 8;
+// Elements a lane takes at once with vectors: eight, and sixteen of 8-bit states beside 16-bit
+// parameters and gradients (W: bytes of the parameter or master weight and the gradient).
+template <bool FP8, int W> constexpr int kLaneElems = FP8 && W <= 4 ? 16 : 8;
 
-template <bool FP8, typename P, typename G>
-__device__ __forceinline__ void step_vector(const AdamArgs& a, const StepScalars& s, float keep, P* param, const G* grad, uint64_t si) {
-  constexpr int E = kLaneElems<FP8>;
-  F2 g[E / 2], p[E / 2], r[E / 2];
-  States<FP8, E> st;
-  load_pairs<E>(grad, g);
-  if (a.master) load_pairs<E>(a.master + si, p);
-  else load_pairs<E>(param, p);
-  st.load(a, si);
-  #pragma unroll
-  for (int i = 0; i < E / 2; ++i) update2(s, keep, g[i], st.m[i], st.v[i], p[i], r[i]);
-  if (a.master) store_pairs<E>(a.master + si, p);
-  store_pairs<E>(param, p);
-  st.store(a, si, r);
-}
+// One lane's vectors of a step; V: what the new value is computed from, the parameter's type or fp32.
+template <bool FP8, typename P, typename G, typename V>
+struct Lane {
+  static constexpr int E = kLaneElems<FP8, sizeof(V) + sizeof(G)>;
+  RawVec<V, E> p;
+  RawVec<G, E> g;
+  RawStates<FP8, E> st;
 
-// A block of 128 elements, four a lane: parameters and gradients one by one, for tensors at odd
-// addresses (FULL) and for the ends of tensors.  The states keep their vectors.
-template <bool FP8, bool FULL, typename P, typename G>
-__device__ __forceinline__ void step_block(const AdamArgs& a, const StepScalars& s, float keep, P* param, const G* grad, uint64_t si, uint32_t left) {
-  float g[4], p[4];
-  States<FP8, 4> st;
-  #pragma unroll
-  for (int k = 0; k < 4; ++k) g[k] = FULL || k < left ? to_f32(grad[k]) : 0.f;
-  if (a.master) {
-    F2 w[2];
-    load_pairs<4>(a.master + si, w);
-    p[0] = w[0].x, p[1] = w[0].y, p[2] = w[1].x, p[3] = w[1].y;
-  } else {
-    #pragma unroll
-    for (int k = 0; k < 4; ++k) p[k] = FULL || k < left ? to_f32(param[k]) : 0.f;
+  __device__ __forceinline__ void load(const AdamArgs& a, const V* from, const G* grad, uint64_t si) {
+    g.load(grad);
+    p.load(from);
+    st.load(a, si);
   }
-  st.load(a, si);
-  F2 w[2] = {{p[0], p[1]}, {p[2], p[3]}}, r[2];
-  update2(s, keep, {g[0], g[1]}, st.m[0], st.v[0], w[0], r[0]);
-  update2(s, keep, {g[2], g[3]}, st.m[1], st.v[1], w[1], r[1]);
-  if (a.master) store_pairs<4>(a.master + si, w);
-  p[0] = w[0].x, p[1] = w[0].y, p[2] = w[1].x, p[3] = w[1].y;
+
+  __device__ __forceinline__ void step(const AdamArgs& a, const StepScalars& s, float keep, P* param, V* from, uint64_t si) const {
+    F2 grad[E / 2], value[E / 2], r[E / 2];
+    States<FP8, E> states;
+    g.pairs(grad);
+    p.pairs(value);
+    states.decode(st);
+    #pragma unroll
+    for (int i = 0; i < E / 2; ++i) update2(s, keep, grad[i], states.m[i], states.v[i], value[i], r[i]);
+    if constexpr (!std::is_same_v<P, V>) store_pairs<E>(from, value);
+    store_pairs<E>(param, value);
+    states.store(a, si, r);
+  }
+};
+
+// Copies of a warp's next vectors into its own shared memory, kStages steps ahead (8-bit states).
+// The arithmetic of sixteen elements needs the registers that a register prefetch would take.
+// Lanes copy 16 bytes side by side (every sector once) and read back their own elements, so a
+// warp's barrier stands after the wait for the copies and before a stage is filled again.
+constexpr int kStages = 3, kMaxSlots = 6;
+constexpr size_t kStageBytes = (size_t)kStages * kMaxSlots * kThreads * 16;
+
+__device__ __forceinline__ void copy_async16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+
+template <typename P, typename G, typename V>
+struct Ahead {
+  using L = Lane<true, P, G, V>;
+  static constexpr int E = L::E, kP = E * (int)sizeof(V) / 16, kG = E * (int)sizeof(G) / 16;
+  static_assert(kP + kG + E / 8 <= kMaxSlots);
+  float ms[kStages], vs[kStages];
+
+  // the warp's part of a stage, 512 bytes a slot
+  __device__ __forceinline__ static uint4* slot(int stage, int i) {
+    extern __shared__ uint4 slots[];
+    return slots + ((stage * kWarps + (threadIdx.x >> 5)) * kMaxSlots + i) * 32;
+  }
+  __device__ __forceinline__ static uint32_t at(int stage, int i) {
+    return (uint32_t)__cvta_generic_to_shared(slot(stage, i) + (threadIdx.x & 31));
+  }
+
+  // from, grad, si: the warp's first element
+  __device__ __forceinline__ void issue(int stage, const AdamArgs& a, const V* from, const G* grad, uint64_t si) {
+    const uint32_t lane = threadIdx.x & 31;
+    #pragma unroll
+    for (int i = 0; i < kP; ++i) copy_async16(at(stage, i), reinterpret_cast<const uint4*>(from) + 32 * i + lane);
+    #pragma unroll
+    for (int i = 0; i < kG; ++i) copy_async16(at(stage, kP + i), reinterpret_cast<const uint4*>(grad) + 32 * i + lane);
+    const uint8_t *m = reinterpret_cast<const uint8_t*>(a.m) + si, *v = reinterpret_cast<const uint8_t*>(a.v) + si;
+    if constexpr (E == 16) {
+      copy_async16(at(stage, kP + kG), m + 16 * lane);
+      copy_async16(at(stage, kP + kG + 1), v + 16 * lane);
+    } else {                            // 256 bytes each: half a slot
+      copy_async16(at(stage, kP + kG), lane < 16 ? m + 16 * lane : v + 16 * (lane - 16));
+    }
+    ms[stage] = a.m_scale[(si + lane * E) / kStateBlock];
+    vs[stage] = a.v_scale[(si + lane * E) / kStateBlock];
+  }
+
+  __device__ __forceinline__ L take(int stage) const {
+    L l;
+    const uint32_t lane = threadIdx.x & 31;
+    #pragma unroll
+    for (int i = 0; i < kP; ++i) put(l.p.w + 4 * i, slot(stage, 0)[kP * lane + i]);
+    #pragma unroll
+    for (int i = 0; i < kG; ++i) put(l.g.w + 4 * i, slot(stage, kP)[kG * lane + i]);
+    if constexpr (E == 16) {
+      put(l.st.m, slot(stage, kP + kG)[lane]);
+      put(l.st.v, slot(stage, kP + kG + 1)[lane]);
+    } else {
+      const uint2 *m = reinterpret_cast<const uint2*>(slot(stage, kP + kG)) + lane, *v = m + 32;
+      l.st.m[0] = m->x, l.st.m[1] = m->y, l.st.v[0] = v->x, l.st.v[1] = v->y;
+    }
+    l.st.ms = ms[stage];
+    l.st.vs = vs[stage];
+    return l;
+  }
+
+ private:
+  __device__ __forceinline__ static void put(uint32_t* w, uint4 v) { w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w; }
+};
+
+// Elements a warp takes at once of tensors at odd addresses: as many as the registers hold.
+template <bool FP8> constexpr uint32_t kOddSpan = FP8 ? 512 : 256;
+
+// B blocks of 128 elements, four elements a lane and block: parameters and gradients one by one,
+// for tensors at odd addresses (FULL) and for the ends of tensors.  The states keep their vectors.
+// All loads come before the first store, so that several blocks' are in flight.
+template <bool FP8, int B, bool FULL, typename P, typename G, typename V>
+__device__ __forceinline__ void step_blocks(const AdamArgs& a, const StepScalars& s, float keep, P* param, V* from, const G* grad, uint64_t si,
+                                            uint32_t left) {
+  constexpr bool kMaster = !std::is_same_v<P, V>;
+  F2 g[B][2], p[B][2], r[2];
+  RawStates<FP8, 4> raw[B];
   #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (FULL || k < left) param[k] = from_f32<P>(p[k]);
-  st.store(a, si, r);
+  for (int b = 0; b < B; ++b) {
+    const uint32_t at = b * kStateBlock;
+    auto one = [&](auto* from, uint32_t k) { return FULL || k < left ? to_f32(from[at + k]) : 0.f; };
+    g[b][0] = {one(grad, 0), one(grad, 1)};
+    g[b][1] = {one(grad, 2), one(grad, 3)};
+    if constexpr (kMaster) {
+      load_pairs<4>(from + at, p[b]);
+    } else {
+      p[b][0] = {one(param, 0), one(param, 1)};
+      p[b][1] = {one(param, 2), one(param, 3)};
+    }
+    raw[b].load(a, si + at);
+  }
+  #pragma unroll
+  for (int b = 0; b < B; ++b) {
+    const uint32_t at = b * kStateBlock;
+    States<FP8, 4> st;
+    st.decode(raw[b]);
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) update2(s, keep, g[b][i], st.m[i], st.v[i], p[b][i], r[i]);
+    if constexpr (kMaster) store_pairs<4>(from + at, p[b]);
+    #pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (FULL || k < left) param[at + k] = from_f32<P>(k & 1 ? p[b][k / 2].y : p[b][k / 2].x);
+    st.store(a, si + at, r);
+  }
 }
 
-template <bool FP8, typename P, typename G>
-__device__ __forceinline__ void step_chunk(const AdamArgs& a, const StepScalars& s, float keep, const AdamTensor& t, uint64_t grad,
+template <bool FP8, typename P, typename G, typename V>
+__device__ __forceinline__ void step_chunk(const AdamArgs& a, const StepScalars& s, float keep, const AdamTensor& t, V* from, uint64_t grad,
                                            uint64_t begin, uint64_t end) {
-  constexpr uint32_t kSpan = 32 * kLaneElems<FP8>;        // elements of a warp's step
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  using L = Lane<FP8, P, G, V>;
+  constexpr uint32_t kSpan = 32 * L::E, kStep = kWarps * kSpan;     // elements a warp, a CTA takes at once
+  const uint32_t lane = threadIdx.x & 31, off = lane * L::E;
   P* param = reinterpret_cast<P*>(t.param);
   const G* gp = reinterpret_cast<const G*>(grad);
   const bool aligned = ((t.param | grad) & 31) == 0;
-  for (uint64_t i = begin + warp * kSpan; i < end; i += kWarps * kSpan) {
-    if (aligned && i + kSpan <= end) {
-      const uint64_t j = i + lane * kLaneElems<FP8>;
-      step_vector<FP8>(a, s, keep, param + j, gp + j, t.state + j);
-    } else {
-      for (uint64_t b = i; b < i + kSpan && b < end; b += kStateBlock) {
-        const uint64_t j = b + lane * 4;
-        if (b + kStateBlock <= end) step_block<FP8, true>(a, s, keep, param + j, gp + j, t.state + j, 4);
-        else step_block<FP8, false>(a, s, keep, param + j, gp + j, t.state + j, j < end ? (uint32_t)(end - j) : 0u);
+  const uint32_t span = aligned ? kSpan : kOddSpan<FP8>;
+  uint64_t i = begin + (threadIdx.x >> 5) * span;
+  if (!aligned) {
+    #pragma unroll 1
+    for (; i + kOddSpan<FP8> <= end; i += kWarps * kOddSpan<FP8>) {
+      const uint64_t j = i + lane * 4;
+      step_blocks<FP8, (int)(kOddSpan<FP8> / kStateBlock), true>(a, s, keep, param + j, from + j, gp + j, t.state + j, 4);
+    }
+  } else if constexpr (FP8) {
+    Ahead<P, G, V> ahead;
+    #pragma unroll
+    for (int k = 0; k < kStages; ++k) {
+      const uint64_t j = i + k * kStep;
+      if (j + kSpan <= end) ahead.issue(k, a, from + j, gp + j, t.state + j);
+      copies_commit();
+    }
+    while (i + kSpan <= end) {
+      #pragma unroll
+      for (int k = 0; k < kStages; ++k) {
+        if (i + kSpan > end) break;
+        copies_wait();
+        __syncwarp();
+        ahead.take(k).step(a, s, keep, param + i + off, from + i + off, t.state + i + off);
+        __syncwarp();
+        const uint64_t j = i + kStages * kStep;
+        if (j + kSpan <= end) ahead.issue(k, a, from + j, gp + j, t.state + j);
+        copies_commit();
+        i += kStep;
       }
     }
+  } else {
+    #pragma unroll 1
+    for (; i + kSpan <= end; i += kStep) {
+      const uint64_t j = i + off;
+      L cur;
+      cur.load(a, from + j, gp + j, t.state + j);
+      cur.step(a, s, keep, param + j, from + j, t.state + j);
+    }
+  }
+  // what is left of the tensor is less than a span, of one warp
+  const uint64_t stop = min(i + span, end);
+  #pragma unroll 1
+  for (; i < stop; i += kStateBlock) {
+    const uint64_t j = i + lane * 4;
+    step_blocks<FP8, 1, false>(a, s, keep, param + j, from + j, gp + j, t.state + j, j < end ? (uint32_t)min(end - j, (uint64_t)4) : 0u);
   }
 }
 
-template <bool FP8, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const AdamArgs a, const __grid_constant__ Grads<N> g) {
+template <bool FP8, bool MASTER, typename P, typename G>
+__device__ __forceinline__ void step_chunk_of(const AdamArgs& a, const StepScalars& s, float keep, const AdamTensor& t, uint64_t grad,
+                                              uint64_t begin, uint64_t end) {
+  if constexpr (MASTER && sizeof(P) == 2) step_chunk<FP8, P, G, float>(a, s, keep, t, a.master + t.state, grad, begin, end);
+  else step_chunk<FP8, P, G, P>(a, s, keep, t, reinterpret_cast<P*>(t.param), grad, begin, end);
+}
+
+template <bool FP8, bool MASTER, int N>
+__global__ void __launch_bounds__(kThreads, kAdamCtas<FP8>) adamw_kernel(const AdamArgs a, const __grid_constant__ Grads<N> g) {
   __shared__ StepScalars shared;
   __shared__ double red[kWarps];
   double sum_sq = 0.0;
@@ -280,11 +443,11 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const AdamArgs a, const
     const AdamTensor t = a.tensors[ch.tensor];
     const float keep = (float)(1.0 - (double)s.lr * t.weight_decay);
     const uint64_t begin = (uint64_t)ch.chunk * a.chunk, end = begin + a.chunk < t.numel ? begin + a.chunk : t.numel;
-    if (t.dtype == DT_F32) step_chunk<FP8, float, float>(a, s, keep, t, grad, begin, end);
-    else if (t.dtype == DT_BF16 && (gp & 1)) step_chunk<FP8, __nv_bfloat16, float>(a, s, keep, t, grad, begin, end);
-    else if (t.dtype == DT_BF16) step_chunk<FP8, __nv_bfloat16, __nv_bfloat16>(a, s, keep, t, grad, begin, end);
-    else if (gp & 1) step_chunk<FP8, __half, float>(a, s, keep, t, grad, begin, end);
-    else step_chunk<FP8, __half, __half>(a, s, keep, t, grad, begin, end);
+    if (t.dtype == DT_F32) step_chunk_of<FP8, MASTER, float, float>(a, s, keep, t, grad, begin, end);
+    else if (t.dtype == DT_BF16 && (gp & 1)) step_chunk_of<FP8, MASTER, __nv_bfloat16, float>(a, s, keep, t, grad, begin, end);
+    else if (t.dtype == DT_BF16) step_chunk_of<FP8, MASTER, __nv_bfloat16, __nv_bfloat16>(a, s, keep, t, grad, begin, end);
+    else if (gp & 1) step_chunk_of<FP8, MASTER, __half, float>(a, s, keep, t, grad, begin, end);
+    else step_chunk_of<FP8, MASTER, __half, __half>(a, s, keep, t, grad, begin, end);
   }
   // the last CTA of a step's last launch advances the clock; all others have read it by then
   if (g.last && threadIdx.x == 0) {
@@ -298,7 +461,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const AdamArgs a, const
   }
 }
 
-template <bool FP8, int N>
+template <bool FP8, bool MASTER, int N>
 cudaError_t adamw_launch_n(const AdamArgs& a, const uint64_t* grads, const uint32_t* chunk_start, uint32_t first, uint32_t n,
                            int sms, cudaStream_t stream) {
   Grads<N> g;
@@ -307,20 +470,26 @@ cudaError_t adamw_launch_n(const AdamArgs& a, const uint64_t* grads, const uint3
   g.first_chunk = chunk_start[first];
   g.n_chunks = chunk_start[first + n] - g.first_chunk;
   g.last = first + n == a.n_tensors;
-  const uint32_t cap = (uint32_t)sms * 8u;
+  // 8-bit states: all CTAs resident at once; fp32 states: twice as many as are, 1 % faster
+  const uint32_t cap = (uint32_t)(sms * (FP8 ? kAdamCtas<FP8> : 2 * kAdamCtas<FP8>));
   const uint32_t grid = g.n_chunks < 1 ? 1 : g.n_chunks < cap ? g.n_chunks : cap;
-  adamw_kernel<FP8, N><<<grid, kThreads, 0, stream>>>(a, g);
+  const size_t shared = FP8 ? kStageBytes : 0;
+  if (FP8) {
+    const cudaError_t e = cudaFuncSetAttribute(adamw_kernel<FP8, MASTER, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+    if (e != cudaSuccess) return e;
+  }
+  adamw_kernel<FP8, MASTER, N><<<grid, kThreads, shared, stream>>>(a, g);
   return cudaGetLastError();
 }
 
-template <bool FP8>
+template <bool FP8, bool MASTER>
 cudaError_t adamw_launch(const AdamArgs& a, const uint64_t* grads, const uint32_t* chunk_start, int sms, cudaStream_t stream) {
   for (uint32_t first = 0; first < a.n_tensors; first += kGradsPerLaunch) {
     const uint32_t n = a.n_tensors - first < kGradsPerLaunch ? a.n_tensors - first : kGradsPerLaunch;
     // launch arguments are copied per launch: a small optimizer does not pay for thousands of addresses
-    const cudaError_t e = n <= 64 ? adamw_launch_n<FP8, 64>(a, grads, chunk_start, first, n, sms, stream)
-                          : n <= 512 ? adamw_launch_n<FP8, 512>(a, grads, chunk_start, first, n, sms, stream)
-                                     : adamw_launch_n<FP8, kGradsPerLaunch>(a, grads, chunk_start, first, n, sms, stream);
+    const cudaError_t e = n <= 64 ? adamw_launch_n<FP8, MASTER, 64>(a, grads, chunk_start, first, n, sms, stream)
+                          : n <= 512 ? adamw_launch_n<FP8, MASTER, 512>(a, grads, chunk_start, first, n, sms, stream)
+                                     : adamw_launch_n<FP8, MASTER, kGradsPerLaunch>(a, grads, chunk_start, first, n, sms, stream);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -424,7 +593,9 @@ uint32_t partial_sums_launch(NormTensor* t, uint32_t n, double* partial, int sms
 }  // namespace
 
 cudaError_t launch_adamw(const AdamArgs& a, const uint64_t* grads, const uint32_t* chunk_start, int sms, cudaStream_t stream) {
-  return a.m_scale ? adamw_launch<true>(a, grads, chunk_start, sms, stream) : adamw_launch<false>(a, grads, chunk_start, sms, stream);
+  const auto launch = a.m_scale ? (a.master ? adamw_launch<true, true> : adamw_launch<true, false>)
+                                : (a.master ? adamw_launch<false, true> : adamw_launch<false, false>);
+  return launch(a, grads, chunk_start, sms, stream);
 }
 
 uint64_t partial_sums_size(uint32_t n, int sms) {

@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <type_traits>
 
 namespace wb {
 
@@ -33,6 +34,15 @@ __device__ __forceinline__ uint4 load16(const void* p) {
 __device__ __forceinline__ void store16(void* p, uint4 v) {
   asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ uint2 load8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store8(void* p, uint2 v) {
+  asm volatile("st.global.v2.b32 [%0], {%1,%2};" ::"l"(p), "r"(v.x), "r"(v.y) : "memory");
+}
+
 template <typename T> constexpr int kVecN = 32 / (int)sizeof(T);
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -113,29 +123,41 @@ __device__ __forceinline__ Vec32 pack(const F2 (&x)[kVecN<T> / 2]) {
   return v;
 }
 
-// E consecutive elements as pairs of fp32, in the widest vectors that they fill; p is aligned to
-// them, or to 32 bytes where they are longer.
-template <int E, typename T>
-__device__ __forceinline__ void load_pairs(const T* p, F2 (&x)[E / 2]) {
-  constexpr int kBytes = E * (int)sizeof(T);
-  if constexpr (kBytes >= 32) {
-    #pragma unroll
-    for (int k = 0; k < kBytes / 32; ++k) {
-      F2 part[kVecN<T> / 2];
-      unpack<T>(load32(p + k * kVecN<T>), part);
+// E consecutive elements of one lane as they come from memory, in the widest vectors that they fill;
+// the address is aligned to them, or to 32 bytes where they are longer.
+template <typename T, int E>
+struct RawVec {
+  static constexpr int kWords = E * (int)sizeof(T) / 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWords >= 8) {
       #pragma unroll
-      for (int i = 0; i < kVecN<T> / 2; ++i) x[k * (kVecN<T> / 2) + i] = part[i];
+      for (int k = 0; k < kWords / 8; ++k) {
+        const Vec32 v = load32(p + k * kVecN<T>);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) w[8 * k + i] = v.w[i];
+      }
+    } else {
+      static_assert(kWords == 4);
+      const uint4 v = load16(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     }
-  } else {
-    static_assert(kBytes == 16);
-    const uint4 v = load16(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  }
+  __device__ __forceinline__ void pairs(F2 (&x)[E / 2]) const {
     #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
       if constexpr (sizeof(T) == 4) x[i] = {__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])};
       else x[i] = unpack2(w[i], T{});
     }
   }
+};
+
+template <int E, typename T>
+__device__ __forceinline__ void load_pairs(const T* p, F2 (&x)[E / 2]) {
+  RawVec<T, E> v;
+  v.load(p);
+  v.pairs(x);
 }
 
 template <int E, typename T>

@@ -102,7 +102,8 @@ class AdamW:
     def states(self) -> dict[str, torch.Tensor]:
         """The flat state buffers: ``exp_avg`` and ``exp_avg_sq`` (fp32), or ``exp_avg`` and
         ``rms`` (e4m3, the root of the second moment) with ``exp_avg_scale`` and ``rms_scale``;
-        ``master`` with master weights.  They are the optimizer's own, not copies."""
+        ``master`` with master weights (the slices of fp32 parameters are not used).  They are the
+        optimizer's own, not copies."""
         p = self._program
         if self.state_bits == "fp8":
             out = {"exp_avg": p.exp_avg, "exp_avg_scale": p.exp_avg_scale, "rms": p.second, "rms_scale": p.second_scale}
