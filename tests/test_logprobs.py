@@ -109,7 +109,7 @@ def _inputs(rows, cols, dtype, seed=0, std=3.0, vocab=None):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (5, 31), (2, 33), (7, 255), (4, 1000), (3, 1001), (2, 2048), (2, 2049), (3, 4097),
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (5, 31), (2, 33), (7, 255), (4, 1000), (3, 1001), (2, 2048), (2, 2049), (3, 4097), (2400, 1500), (2400, 9001),
                                         (33, 5003), (1, 128256), (2, 151937)])
 def test_sizes_and_types(dtype, rows, vocab):
     x, t = _inputs(rows, vocab, dtype)
@@ -368,6 +368,8 @@ def test_refusals():
         refused("top_k must be", top_k=k)
     refused("top_k must be between 0 and 32", torch.randn(4, 100), top_k=33)
     refused("top_k must be between 0 and 3", vocab=3, top_k=4)
+    refused("at most 2097152 columns", torch.empty(1, 2 ** 21 + 1, dtype=torch.float16), torch.zeros(1, dtype=torch.long), top_k=1)
+    refused("2\\^30 columns", torch.empty(1, dtype=torch.float16).expand(1, 2 ** 30 + 1), torch.zeros(1, dtype=torch.long))
     for v in (0.0, -1.0, math.nan, math.inf, 1e-60):
         refused("temperature", temperature=v)
     refused("contiguous", torch.randn(10, 4).t())

@@ -211,8 +211,8 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::
   if (tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1))
     bad("token_logprobs: tokens of shape " + shape_of(tokens) + " do not match logits of shape " + shape_of(logits));
   if (vocab < 1 || vocab > cols) bad("token_logprobs: vocab must be between 1 and the logits' " + std::to_string(cols) + " columns");
-  if (cols > std::numeric_limits<int32_t>::max() || tokens.numel() >= std::numeric_limits<int32_t>::max())
-    bad("token_logprobs: at most 2^31 - 1 columns and rows");
+  if (cols > wb::kLogprobMaxColumns || tokens.numel() >= std::numeric_limits<int32_t>::max())
+    bad("token_logprobs: at most 2^30 columns and 2^31 - 2 rows");
   if (!(temperature > 0) || !std::isfinite(temperature) || !std::isfinite((float)(1.0 / temperature)) || (float)(1.0 / temperature) == 0.f)
     bad("token_logprobs: the temperature must be positive and finite");
   if (top_k < 0 || top_k > wb::kLogprobMaxTop || top_k > vocab)

@@ -16,9 +16,13 @@
 // A CTA of eight warps takes a row; where rows are few, a cluster of CTAs shares one and joins
 // through distributed shared memory (no workspace, no second launch).
 //
-// Alternatives: a tile's columns are consecutive, so by (logit descending, column ascending) the
-// k first columns lie in the k first tiles ranked by (their largest logit, tile).  The pass leaves
-// each tile's maximum in shared memory; k tiles are picked, read once more and searched.
+// Alternatives: by (logit descending, column ascending) the k first columns lie in the k first groups
+// of consecutive columns ranked by (their largest logit, their place).  The pass leaves each tile's
+// maximum in shared memory; the k first tiles are found by counting how many come before each, and
+// read once more: the columns that reach the least of the k maxima (few more than k) are ranked by
+// counting, too.  Only where ties or a short row make those many does a selection among the tiles'
+// 32-byte vectors come between, which bounds them by k vectors.  (Taking the largest k times over
+// cost 1 us an alternative; a binary search for the k-th maximum 6 us.)
 #include "wb_logprobs.h"
 
 #include <cooperative_groups.h>
@@ -118,15 +122,26 @@ __device__ __forceinline__ RowStats warp_join(RowStats t, float c2) {
   return {t.m, warp_sum(t.s), warp_sum(t.a)};
 }
 
-// A tile that the row does not fill, element by element; what lies outside the row reads as -inf.
+template <typename T> constexpr uint32_t kNegInf = sizeof(T) == 4 ? 0xff800000u : 0;
+template <> constexpr uint32_t kNegInf<__nv_bfloat16> = 0xff80u;
+template <> constexpr uint32_t kNegInf<__half> = 0xfc00u;
+
+// A lane's vector of columns j0 .. j0 + N - 1; what lies outside the row reads as -inf.
 template <typename T>
-__device__ __forceinline__ void load_edge(const T* x, uint32_t vocab, int64_t j0, F2 (&v)[kVecN<T> / 2]) {
+__device__ __forceinline__ Vec32 load_vec(const T* x, uint32_t vocab, int32_t j0) {
+  constexpr int N = kVecN<T>;
+  Vec32 v;
+  if (j0 >= 0 && (uint32_t)j0 + N <= vocab) return load32(x + j0);
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+  uint32_t e[N];
   #pragma unroll
-  for (int i = 0; i < kVecN<T>; ++i) {
-    const int64_t j = j0 + i;
-    const float f = j >= 0 && j < (int64_t)vocab ? to_f32(x[j]) : -kInf;
-    if (i & 1) v[i / 2].y = f; else v[i / 2].x = f;
+  for (int i = 0; i < N; ++i) {
+    const int32_t j = j0 + i;
+    e[i] = j >= 0 && (uint32_t)j < vocab ? (uint32_t) reinterpret_cast<const Bits*>(x)[j] : kNegInf<T>;
   }
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) v.w[i] = sizeof(T) == 4 ? e[i] : e[2 * i % N] | e[(2 * i + 1) % N] << 16;
+  return v;
 }
 
 struct RowResult { float m, ln, entropy; bool empty; };
@@ -144,10 +159,14 @@ __device__ __forceinline__ float logprob(const RowResult& t, float x, float inv_
   return t.empty ? -kInf : (x - t.m) * inv_temp - t.ln;
 }
 
+// The token's logit, loaded before the row: its latency passes under the row's.
 template <typename T>
-__device__ __forceinline__ void write_row(const LogprobRows& in, const LogprobOut& out, uint32_t r, const T* x, int64_t tok,
-                                          const RowResult& t) {
-  out.logprobs[r] = tok >= 0 && tok < (int64_t)in.vocab ? logprob(t, to_f32(x[tok]), in.inv_temp) : kNaN;
+__device__ __forceinline__ float token_logit(const LogprobRows& in, const T* x, int64_t tok) {
+  return tok >= 0 && tok < (int64_t)in.vocab ? to_f32(x[tok]) : kNaN;
+}
+
+__device__ __forceinline__ void write_row(const LogprobRows& in, const LogprobOut& out, uint32_t r, int64_t tok, float xt, const RowResult& t) {
+  out.logprobs[r] = tok >= 0 && tok < (int64_t)in.vocab ? logprob(t, xt, in.inv_temp) : kNaN;
   out.entropy[r] = t.entropy;
   if (out.stats) {
     out.stats[2 * (int64_t)r] = t.m;
@@ -161,7 +180,26 @@ __device__ __forceinline__ void write_ignored(const LogprobOut& out, uint32_t r)
   if (out.stats) out.stats[2 * (int64_t)r] = out.stats[2 * (int64_t)r + 1] = 0.f;
 }
 
-// Tiles [first, first + step, ...) below `end` of a row into this lane's statistics; two at a time,
+// Keys of 16-bit types differ in their upper bits only.
+template <typename T> constexpr int kKeyShift = 0;
+template <> constexpr int kKeyShift<__nv_bfloat16> = 16;
+template <> constexpr int kKeyShift<__half> = 13;
+
+// A tile's maximum as it is kept: 16-bit types have room for the tile below the key, lower tiles first.
+template <typename T>
+__device__ __forceinline__ uint32_t tile_key(uint32_t key, uint32_t tile) {
+  constexpr uint32_t kMask = (1u << kKeyShift<T>) - 1;
+  return kMask ? (key & ~kMask) | (kMask - tile) : key;
+}
+static_assert(kLogprobMaxTopVocab / kTile<__half> + 1 < 1u << kKeyShift<__half>);
+
+// Whether tile j comes before tile i.
+template <typename T>
+__device__ __forceinline__ uint32_t tile_before(uint32_t key_j, uint32_t j, uint32_t key_i, uint32_t i) {
+  return kKeyShift<T> ? key_j > key_i : key_j + (j < i) > key_i;
+}
+
+// Tiles first, first + step, ... below `end` of a row into this lane's statistics; two at a time,
 // so that the second's load runs under the first's arithmetic.  tops: each tile's largest, as a key.
 template <typename T, bool TOP>
 __device__ __forceinline__ Stats walk(const T* x, uint32_t vocab, uint32_t mis, uint32_t first, uint32_t step, uint32_t end,
@@ -169,142 +207,218 @@ __device__ __forceinline__ Stats walk(const T* x, uint32_t vocab, uint32_t mis, 
   constexpr int N = kVecN<T>, kDepth = 2;
   const uint32_t lane = threadIdx.x & 31;
   Stats st;
-  const T* aligned = x - mis;
-  // full tiles: those that begin at or behind the row's start and end at or before its end
-  const uint32_t full_from = mis ? 1 : 0, full_to = (mis + vocab) / kTile<T>;
   for (uint32_t t = first; t < end; t += kDepth * step) {
     Vec32 raw[kDepth];
-    bool full[kDepth];
     #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
       const uint32_t k = t + u * step;
-      full[u] = k >= full_from && k < full_to && k < end;
-      if (full[u]) raw[u] = load32(aligned + (int64_t)k * kTile<T> + lane * N);
+      if (k < end) raw[u] = load_vec(x, vocab, (int32_t)(k * kTile<T> + lane * N - mis));
     }
     #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
       const uint32_t k = t + u * step;
       if (k >= end) break;
       F2 v[N / 2];
-      if (full[u]) unpack<T>(raw[u], v);
-      else load_edge(x, vocab, (int64_t)k * kTile<T> + lane * N - mis, v);
+      unpack<T>(raw[u], v);
       const float top = tile_max(v);
       accumulate(st, v, top, c2);
       if constexpr (TOP) {
-        const uint32_t key = __reduce_max_sync(kFullWarp, order_key(top));
-        if (lane == 0) tops[k - base] = key;
+        const uint32_t key = __reduce_max_sync(kFullWarp, order_key(fmaxf(top, -kInf)));
+        if (lane == 0) tops[k - base] = tile_key<T>(key, k - base);
       }
     }
   }
   return st;
 }
 
-// Many short rows: a warp each.
+// Many short rows: a warp takes one after another; the next row's token is under way meanwhile.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) logprobs_warp_kernel(const LogprobRows in, const LogprobOut out) {
-  const uint32_t r = blockIdx.x * kWarps + threadIdx.x / 32;
-  if (r >= in.rows) return;
-  const int64_t tok = token_of(in, r);
-  if (tok == in.ignore_index) {
-    if (threadIdx.x % 32 == 0) write_ignored(out, r);
-    return;
-  }
-  const T* x = row_ptr<T>(in, r);
+  const uint32_t warps = gridDim.x * kWarps, lane = threadIdx.x & 31;
   const float c2 = in.inv_temp * kLog2e;
-  const uint32_t mis = misaligned(x), tiles = (mis + in.vocab + kTile<T> - 1) / kTile<T>;
-  const Stats st = walk<T, false>(x, in.vocab, mis, 0, 1, tiles, 0, c2, nullptr);
-  const RowStats t = warp_join({st.m, st.s.x + st.s.y, st.a.x + st.a.y}, c2);
-  if (threadIdx.x % 32 == 0) write_row(in, out, r, x, tok, finish(t));
+  uint32_t r = blockIdx.x * kWarps + threadIdx.x / 32;
+  int64_t next = r < in.rows ? token_of(in, r) : 0;
+  for (; r < in.rows; r += warps) {
+    const int64_t tok = next;
+    if (in.rows - r > warps) next = token_of(in, r + warps);
+    if (tok == in.ignore_index) {
+      if (lane == 0) write_ignored(out, r);
+      continue;
+    }
+    const T* x = row_ptr<T>(in, r);
+    const float xt = token_logit(in, x, tok);
+    const uint32_t mis = misaligned(x), tiles = (mis + in.vocab + kTile<T> - 1) / kTile<T>;
+    const Stats st = walk<T, false>(x, in.vocab, mis, 0, 1, tiles, 0, c2, nullptr);
+    const RowStats t = warp_join({st.m, st.s.x + st.s.y, st.a.x + st.a.y}, c2);
+    if (lane == 0) write_row(in, out, r, tok, xt, finish(t));
+  }
 }
 
 // -- alternatives ---------------------------------------------------------------------------------
-// The largest (key, lowest index) over the warp; key 0: none.
-__device__ __forceinline__ bool warp_best(uint32_t key, uint32_t idx, uint32_t& best_key, uint32_t& best_idx) {
-  best_key = __reduce_max_sync(kFullWarp, key);
-  best_idx = __reduce_min_sync(kFullWarp, key == best_key ? idx : 0xffffffffu);
-  return best_key != 0;
-}
+constexpr uint32_t kTopPerWarp = kLogprobMaxTop / kWarps;                 // selected tiles of one warp
+constexpr uint32_t kMaxCandidates = kLogprobMaxTop * kVecN<__nv_bfloat16>;
 
-// Shared memory of the search, in words: the tiles' maxima, then the keys of the picked tiles.
-template <typename T>
 struct TopShared {
-  uint32_t picked[kLogprobMaxTop], key[kLogprobMaxTop], col[kLogprobMaxTop];   // per picked tile: its best column left
-  uint32_t out_key[kLogprobMaxTop], out_col[kLogprobMaxTop];                   // the result, in order
-  uint32_t n_picked, n_out;
+  uint64_t candidates[kMaxCandidates], out[kLogprobMaxTop];   // key << 32 | ~column
+  uint32_t picked[kLogprobMaxTop], part[2][kWarps];
+  uint32_t n_picked, n_candidates, n_out, least;
 };
 
-// The k first columns of tiles [base, base + n): whole CTA; the result in sh.out_*.
+// A whole number's sum over the CTA; `turn` alternates, so that one barrier a sum is enough.
+__device__ __forceinline__ uint32_t cta_count(uint32_t c, TopShared& sh, uint32_t& turn) {
+  c = __reduce_add_sync(kFullWarp, c);
+  uint32_t* part = sh.part[turn & 1];
+  ++turn;
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = c;
+  __syncthreads();
+  uint32_t sum = 0;
+  #pragma unroll
+  for (int i = 0; i < kWarps; ++i) sum += part[i];
+  return sum;
+}
+
+// Selection of the k first of some groups by (value descending, place ascending): those with a
+// value above `value`, and those with that value up to place `last`.  count(f): how many groups f
+// holds for.  All are selected where there are at most k of value `low` or more.
+struct Selection { uint32_t value, last; };
+
+template <typename Count>
+__device__ Selection select_first(uint32_t k, uint32_t low, uint32_t high, uint32_t places, Count count) {
+  if (count([&](uint32_t v, uint32_t) { return v >= low; }) <= k) return {low, 0xffffffffu};
+  while (low < high) {
+    const uint32_t mid = high - (high - low) / 2;
+    const uint32_t c = count([&](uint32_t v, uint32_t) { return v >= mid; });
+    if (c == k) return {mid, 0xffffffffu};
+    if (c > k) low = mid; else high = mid - 1;
+  }
+  // more than k from `low` on, fewer above it: the first places of that value fill up
+  const uint32_t above = count([&](uint32_t v, uint32_t) { return v > low; });
+  uint32_t from = 0, to = places;
+  while (from < to) {
+    const uint32_t mid = from + (to - from) / 2;
+    if (above + count([&](uint32_t v, uint32_t p) { return v == low && p <= mid; }) >= k) to = mid; else from = mid + 1;
+  }
+  return {low, from};
+}
+
+// Ranks n distinct candidates by counting; the first k go to `out` in order.
+__device__ __forceinline__ void rank_candidates(const uint64_t* c, uint32_t n, uint32_t k, uint64_t* out) {
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t mine = c[i];
+    uint32_t rank = 0;
+    #pragma unroll 4
+    for (uint32_t j = 0; j < n; ++j) rank += c[j] > mine;
+    if (rank < k) out[rank] = mine;
+  }
+}
+
+// The k first columns of tiles [base, base + n), in order, into sh.out.  top: the largest logit of
+// these tiles; tops: each tile's, as a key.
 template <typename T>
-__device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base, uint32_t n, uint32_t k, uint32_t* tops, uint32_t* keys,
-                         TopShared<T>& sh) {
-  constexpr int N = kVecN<T>;
+__device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base, uint32_t n, uint32_t k, float top, const uint32_t* tops,
+                         TopShared& sh) {
+  constexpr int N = kVecN<T>, kShift = kKeyShift<T>;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  if (warp == 0) {                         // pick k tiles by (maximum, lowest tile)
-    uint32_t key = 0, idx = 0xffffffffu, picked = 0;
-    auto scan = [&] {
-      key = 0, idx = 0xffffffffu;
-      for (uint32_t i = lane; i < n; i += 32)
-        if (tops[i] > key) key = tops[i], idx = i;
-    };
-    scan();
-    for (; picked < k; ++picked) {
-      uint32_t bk, bi;
-      if (!warp_best(key, idx, bk, bi)) break;
-      if (lane == 0) sh.picked[picked] = bi;
-      if (idx == bi) {
-        tops[bi] = 0;
-        scan();
-      }
-    }
-    if (lane == 0) sh.n_picked = picked;
-  }
-  __syncthreads();
-  const uint32_t picked = sh.n_picked;
-  for (uint32_t s = warp; s < picked; s += kWarps) {         // their columns' keys, element-major
-    const int64_t j0 = (int64_t)(base + sh.picked[s]) * kTile<T> + lane * N - mis;
-    uint32_t key = 0, col = 0xffffffffu;
-    #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int64_t j = j0 + e;
-      const uint32_t v = j >= 0 && j < (int64_t)vocab ? order_key(to_f32(x[j])) : 0;
-      keys[s * kTile<T> + e * 32 + lane] = v;
-      if (v > key) key = v, col = (uint32_t)j;
-    }
-    uint32_t bk, bc;
-    warp_best(key, col, bk, bc);
-    if (lane == 0) sh.key[s] = bk, sh.col[s] = bc;
-  }
-  __syncthreads();
-  if (warp == 0) {                         // k times the best of the picked tiles' bests
-    uint32_t key = lane < picked ? sh.key[lane] : 0, col = lane < picked ? sh.col[lane] : 0xffffffffu;
-    uint32_t found = 0;
-    for (; found < k; ++found) {
-      uint32_t bk, bc;
-      if (!warp_best(key, col, bk, bc)) break;
-      if (lane == 0) sh.out_key[found] = bk, sh.out_col[found] = bc;
-      const uint32_t s = __ffs(__ballot_sync(kFullWarp, key == bk && col == bc)) - 1;
-      const uint32_t tile = sh.picked[s] + base, at = bc + mis - tile * kTile<T>;
-      uint32_t nk = 0, nc = 0xffffffffu;
+  const uint32_t high = order_key(top) >> kShift;
+  uint32_t turn = 0;
+  const bool counted = n <= 2 * kThreads;
+  if (threadIdx.x == 0) sh.n_picked = sh.n_candidates = 0, sh.least = 1;
+  if (counted) {
+    __syncthreads();
+    const uint32_t i0 = threadIdx.x, i1 = i0 + kThreads;
+    const uint32_t key0 = i0 < n ? tops[i0] : 0, key1 = i1 < n ? tops[i1] : 0;
+    uint32_t rank0 = 0, rank1 = 0;
+    for (uint32_t j = 0; j < n; j += 4) {              // zeros follow the last tile
+      const uint4 q = *reinterpret_cast<const uint4*>(tops + j);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
       #pragma unroll
-      for (int e = 0; e < N; ++e) {        // columns behind the one taken: a lower key, or the same and a higher column
-        const uint32_t v = keys[s * kTile<T> + e * 32 + lane], p = lane * N + e;
-        if ((v < bk || (v == bk && p > at)) && v > nk) nk = v, nc = tile * kTile<T> + p - mis;
+      for (int u = 0; u < 4; ++u) rank0 += tile_before<T>(w[u], j + u, key0, i0);
+      if (n > kThreads) {
+        #pragma unroll
+        for (int u = 0; u < 4; ++u) rank1 += tile_before<T>(w[u], j + u, key1, i1);
       }
-      uint32_t gk, gc;
-      warp_best(nk, nc, gk, gc);
-      if (lane == s) key = gk, col = gc;
     }
-    if (lane == 0) sh.n_out = found;
+    if (i0 < n && rank0 < k) sh.picked[rank0] = base + i0;
+    if (i1 < n && rank1 < k) sh.picked[rank1] = base + i1;
+    if (rank0 == k - 1 && i0 < n) sh.least = key0 >> kShift;
+    if (rank1 == k - 1 && i1 < n) sh.least = key1 >> kShift;
+    if (threadIdx.x == 0) sh.n_picked = min(n, k);
+  } else {
+    const Selection tiles = select_first(k, 1, high, n, [&](auto holds) {
+      uint32_t c = 0;
+      for (uint32_t i = threadIdx.x; i < n; i += kThreads) c += holds(tops[i] >> kShift, i);
+      return cta_count(c, sh, turn);
+    });
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+      const uint32_t v = tops[i] >> kShift;
+      if (v > tiles.value || (v == tiles.value && i <= tiles.last)) sh.picked[atomicAdd(&sh.n_picked, 1u)] = base + i;
+    }
+    if (threadIdx.x == 0) sh.least = tiles.value;
   }
+  __syncthreads();
+  const uint32_t picked = sh.n_picked, least = sh.least;
+  Vec32 raw[kTopPerWarp];
+  uint32_t value[kTopPerWarp];                         // the vectors' largest
+  int32_t j0[kTopPerWarp];
+  #pragma unroll
+  for (uint32_t s = 0; s < kTopPerWarp; ++s) {
+    const uint32_t p = warp + s * kWarps;
+    value[s] = 0;
+    if (p >= picked) continue;
+    j0[s] = (int32_t)(sh.picked[p] * kTile<T> + lane * N - mis);
+    raw[s] = load_vec(x, vocab, j0[s]);
+  }
+  #pragma unroll
+  for (uint32_t s = 0; s < kTopPerWarp; ++s) {
+    if (warp + s * kWarps >= picked || j0[s] + N <= 0 || j0[s] >= (int32_t)vocab) continue;      // no column of the row
+    F2 v[N / 2];
+    unpack<T>(raw[s], v);
+    value[s] = order_key(fmaxf(tile_max(v), -kInf)) >> kShift;
+  }
+  // the columns from `from` on of the vectors that `wanted` takes
+  auto collect = [&](uint32_t from, auto wanted) {
+    #pragma unroll
+    for (uint32_t s = 0; s < kTopPerWarp; ++s) {
+      if (value[s] < from || !value[s] || !wanted(value[s], (uint32_t)(j0[s] + N))) continue;
+      F2 v[N / 2];
+      unpack<T>(raw[s], v);
+      #pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int32_t j = j0[s] + e;
+        const uint32_t key = order_key(e & 1 ? v[e / 2].y : v[e / 2].x);
+        if (j >= 0 && j < (int32_t)vocab && key >> kShift >= from) {
+          const uint32_t at = atomicAdd(&sh.n_candidates, 1u);
+          if (at < kMaxCandidates) sh.candidates[at] = (uint64_t)key << 32 | ~(uint32_t)j;
+        }
+      }
+    }
+    __syncthreads();
+  };
+  collect(least, [](uint32_t, uint32_t) { return true; });
+  if (sh.n_candidates > kMaxCandidates) {              // many columns of one value, or fewer than k tiles
+    // places: the vectors' first columns, counted from one vector before the row's start
+    const Selection vecs = select_first(k, least, high, vocab + N, [&](auto holds) {
+      uint32_t c = 0;
+      #pragma unroll
+      for (uint32_t s = 0; s < kTopPerWarp; ++s) c += value[s] && holds(value[s], (uint32_t)(j0[s] + N));
+      return cta_count(c, sh, turn);
+    });
+    if (threadIdx.x == 0) sh.n_candidates = 0;
+    __syncthreads();
+    collect(vecs.value, [&](uint32_t v, uint32_t place) { return v > vecs.value || place <= vecs.last; });
+  }
+  const uint32_t m = sh.n_candidates;
+  rank_candidates(sh.candidates, m, k, sh.out);
+  if (threadIdx.x == 0) sh.n_out = min(m, k);
   __syncthreads();
 }
 
 // A CTA per row, or a cluster of `splits` CTAs.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) logprobs_row_kernel(const LogprobRows in, const LogprobOut out, const uint32_t splits) {
-  extern __shared__ uint32_t dyn[];                      // TOP: tile maxima, then keys
+  extern __shared__ __align__(16) uint32_t tops[];       // TOP: the tiles' maxima, and zeros up to a multiple of four
   __shared__ RowStats warps[kWarps], mine;
-  __shared__ TopShared<T> sh;
+  __shared__ std::conditional_t<TOP, TopShared, int> shared;
   const uint32_t r = blockIdx.x / splits, split = blockIdx.x % splits;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int64_t tok = token_of(in, r);
@@ -319,54 +433,51 @@ __global__ void __launch_bounds__(kThreads) logprobs_row_kernel(const LogprobRow
     return;
   }
   const T* x = row_ptr<T>(in, r);
+  const float xt = token_logit(in, x, tok);
   const float c2 = in.inv_temp * kLog2e;
   const uint32_t mis = misaligned(x), tiles = (mis + in.vocab + kTile<T> - 1) / kTile<T>;
   const uint32_t per = (tiles + splits - 1) / splits;
   const uint32_t begin = min(split * per, tiles), end = min(begin + per, tiles);
-  const Stats st = walk<T, TOP>(x, in.vocab, mis, begin + warp, kWarps, end, begin, c2, dyn);
+  if (TOP && threadIdx.x < 4) tops[(end - begin) + threadIdx.x] = 0;
+  const Stats st = walk<T, TOP>(x, in.vocab, mis, begin + warp, kWarps, end, begin, c2, tops);
   const RowStats w = warp_join({st.m, st.s.x + st.s.y, st.a.x + st.a.y}, c2);
   if (lane == 0) warps[warp] = w;
   __syncthreads();
-  if (warp == 0) {
-    const RowStats t = warp_join(lane < kWarps ? warps[lane] : RowStats{kLowest, 0.f, 0.f}, c2);
-    if (lane == 0) mine = t;
-  }
-  if constexpr (TOP) find_top(x, in.vocab, mis, begin, end - begin, (uint32_t)out.top_k, dyn, dyn + per, sh);
-  else __syncthreads();
-  RowStats all = mine;
+  // every warp joins the eight: the same operations, the same bits
+  RowStats all = warp_join(lane < kWarps ? warps[lane] : RowStats{kLowest, 0.f, 0.f}, c2);
+  if constexpr (TOP) find_top(x, in.vocab, mis, begin, end - begin, (uint32_t)out.top_k, all.m, tops, shared);
   if (splits > 1) {
     cg::cluster_group cl = cg::this_cluster();
+    if (threadIdx.x == 0) mine = all;
     cl.sync();
-    if (split == 0 && warp == 0) {
+    if (split == 0) {
       all = warp_join(lane < splits ? *cl.map_shared_rank(&mine, lane) : RowStats{kLowest, 0.f, 0.f}, c2);
-      if constexpr (TOP) {
-        // every CTA's list is in order: lane s stands at the head of CTA s's list
-        TopShared<T>* theirs = lane < splits ? cl.map_shared_rank(&sh, lane) : &sh;
-        const uint32_t n = lane < splits ? theirs->n_out : 0;
-        uint32_t at = 0, key = n ? theirs->out_key[0] : 0, col = n ? theirs->out_col[0] : 0xffffffffu;
-        for (uint32_t i = 0; i < (uint32_t)out.top_k; ++i) {
-          uint32_t bk, bc;
-          warp_best(key, col, bk, bc);
-          if (lane == 0) dyn[2 * i] = bk, dyn[2 * i + 1] = bc;     // the maxima are no longer needed
-          if (key == bk && col == bc) {
-            ++at;
-            key = at < n ? theirs->out_key[at] : 0;
-            col = at < n ? theirs->out_col[at] : 0xffffffffu;
-          }
+      if constexpr (TOP) {               // at most 8 * 32 candidates, a thread each
+        const uint32_t k = (uint32_t)out.top_k, s = threadIdx.x / k, i = threadIdx.x % k;
+        uint64_t c = 0;
+        if (s < splits) {
+          const TopShared* theirs = cl.map_shared_rank(&shared, s);
+          if (i < theirs->n_out) c = theirs->out[i];
         }
-        __syncwarp();
-        if (lane < (uint32_t)out.top_k) sh.out_key[lane] = dyn[2 * lane], sh.out_col[lane] = dyn[2 * lane + 1];
-        __syncwarp();
+        if (threadIdx.x == 0) shared.n_candidates = 0;
+        __syncthreads();                 // this CTA's own list has been read, too
+        if (c) shared.candidates[atomicAdd(&shared.n_candidates, 1u)] = c;
+        __syncthreads();
+        rank_candidates(shared.candidates, shared.n_candidates, k, shared.out);
+        __syncthreads();
       }
     }
     cl.sync();                             // the others' shared memory stays until it has been read
   }
   if (split == 0 && warp == 0) {
     const RowResult t = finish(all);
-    if (lane == 0) write_row(in, out, r, x, tok, t);
-    if (TOP && lane < (uint32_t)out.top_k) {
-      out.top_logprobs[(int64_t)r * out.top_k + lane] = logprob(t, key_value(sh.out_key[lane]), in.inv_temp);
-      out.top_ids[(int64_t)r * out.top_k + lane] = sh.out_col[lane];
+    if (lane == 0) write_row(in, out, r, tok, xt, t);
+    if constexpr (TOP) {
+      if (lane < (uint32_t)out.top_k) {
+        const uint64_t c = shared.out[lane];
+        out.top_logprobs[(int64_t)r * out.top_k + lane] = logprob(t, key_value((uint32_t)(c >> 32)), in.inv_temp);
+        out.top_ids[(int64_t)r * out.top_k + lane] = (int64_t)(uint32_t)~(uint32_t)c;
+      }
     }
   }
 }
@@ -405,13 +516,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad_kernel(const LogprobRo
   const bool vectors = misaligned(x) == mis;
   const uint32_t tiles = (mis + g.cols + kTile<T> - 1) / kTile<T>;
   const uint32_t begin = seg * kGradTiles, end = min(begin + kGradTiles, tiles);
-  const uint32_t full_from = mis ? 1 : 0, full_to = vectors ? (mis + in.vocab) / kTile<T> : 0;
   #pragma unroll 2
   for (uint32_t t = begin; t < end; ++t) {
-    if (t >= full_from && t < full_to) {
-      const int64_t j0 = (int64_t)t * kTile<T> + lane * N - mis;
+    const int32_t tile0 = (int32_t)(t * kTile<T> - mis), j0 = tile0 + lane * N;
+    const bool padding = j0 >= (int32_t)in.vocab;
+    if (vectors && j0 >= 0 && (uint32_t)j0 + N <= (padding ? g.cols : in.vocab)) {
       F2 v[N / 2];
-      if (dead) {
+      if (dead || padding) {
         #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[i] = {0.f, 0.f};
       } else {
@@ -428,12 +539,19 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad_kernel(const LogprobRo
       }
       store32(d + j0, pack<T>(v));
     } else {
+      // a lane that passes the row's ends: its own elements; rows that lie otherwise: side by side
+      const int32_t first = vectors ? j0 : tile0 + (int32_t)lane, step = vectors ? 1 : 32;
+      float v[N];
+      #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const int64_t j = (int64_t)t * kTile<T> + e * 32 + lane - mis;
-        if (j < 0 || j >= (int64_t)g.cols) continue;
-        float v = 0.f;
-        if (!dead && j < (int64_t)in.vocab) v = grad2({to_f32(x[j]), 0.f}).x + (j == tok ? onehot : 0.f);
-        d[j] = from_f32<T>(v);
+        const int32_t j = first + e * step;
+        v[e] = !dead && j >= 0 && j < (int32_t)in.vocab ? to_f32(x[j]) : -kInf;
+      }
+      #pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int32_t j = first + e * step;
+        const float y = j < (int32_t)in.vocab && !dead ? grad2({v[e], v[e]}).x + (j == tok ? onehot : 0.f) : 0.f;
+        if (j >= 0 && j < (int32_t)g.cols) d[j] = from_f32<T>(y);
       }
     }
   }
@@ -449,22 +567,22 @@ cudaError_t by_type(uint32_t dtype, F f) {
   }
 }
 
-bool ok(const LogprobRows& in) { return in.rows < 0x7fffffffu && in.vocab >= 1 && in.vocab < 0x7fffffffu && in.inner >= 1; }
-
-// Rows of up to this many columns are read by one warp where nothing else asks for a CTA.
-constexpr uint32_t kWarpRow = 2048;
+bool ok(const LogprobRows& in) { return in.rows < 0x7fffffffu && in.vocab >= 1 && in.vocab <= kLogprobMaxColumns && in.inner >= 1; }
 
 template <typename T>
 cudaError_t launch_rows(const LogprobRows& in, const LogprobOut& out, int sms, cudaStream_t stream) {
   const uint32_t tiles = (in.vocab + kTile<T> - 1) / kTile<T> + 1;
-  if (!out.top_k && in.vocab <= kWarpRow) {
-    logprobs_warp_kernel<T><<<(in.rows + kWarps - 1) / kWarps, kThreads, 0, stream>>>(in, out);
+  // A warp a row: no barrier, no second join.  For rows of up to four tiles, of which a CTA's eight
+  // warps would find no two; and for up to 32 where the rows fill half of the GPU's warps.
+  if (!out.top_k && (tiles <= 5 || (tiles <= 33 && in.rows >= (uint32_t)sms * 16))) {
+    const uint32_t cap = (uint32_t)sms * 4, grid = (in.rows + kWarps - 1) / kWarps;
+    logprobs_warp_kernel<T><<<grid < cap ? grid : cap, kThreads, 0, stream>>>(in, out);
     return cudaGetLastError();
   }
   uint32_t splits = 1;
   while (splits < kMaxSplits && (uint64_t)in.rows * splits * 2 <= (uint64_t)sms * 2 && tiles >= splits * 2 * kWarps) splits *= 2;
   const uint32_t per = (tiles + splits - 1) / splits;
-  const size_t shared = out.top_k ? 4 * (per + (size_t)out.top_k * kTile<T>) : 0;
+  const size_t shared = out.top_k ? 4 * (size_t)per + 16 : 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(in.rows * splits);
   cfg.blockDim = dim3(kThreads);
@@ -477,10 +595,6 @@ cudaError_t launch_rows(const LogprobRows& in, const LogprobOut& out, int sms, c
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   auto kernel = out.top_k ? logprobs_row_kernel<T, true> : logprobs_row_kernel<T, false>;
-  if (shared > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-    if (e != cudaSuccess) return e;
-  }
   return cudaLaunchKernelEx(&cfg, kernel, in, out, splits);
 }
 
@@ -494,7 +608,7 @@ cudaError_t launch_token_logprobs(const LogprobRows& in, const LogprobOut& out, 
 }
 
 cudaError_t launch_token_logprobs_grad(const LogprobRows& in, const LogprobGrad& g, cudaStream_t stream) {
-  if (!ok(in) || g.cols < in.vocab || g.cols >= 0x7fffffffu) return cudaErrorInvalidValue;
+  if (!ok(in) || g.cols < in.vocab || g.cols > kLogprobMaxColumns) return cudaErrorInvalidValue;
   if (in.rows == 0) return cudaSuccess;
   return by_type(in.dtype, [&](auto t) {
     using T = decltype(t);

@@ -8,7 +8,8 @@
 namespace wb {
 
 constexpr int kLogprobMaxTop = 32;
-constexpr uint32_t kLogprobMaxTopVocab = 1u << 22;     // columns with alternatives: the tiles' maxima fit shared memory
+constexpr uint32_t kLogprobMaxColumns = 1u << 30;      // column numbers fit 32 signed bits, a tile past the end too
+constexpr uint32_t kLogprobMaxTopVocab = 1u << 21;     // columns with alternatives: the tiles' maxima fit 32 KiB of shared memory
 
 // Rows of logits: row r = (r / inner, r % inner) starts at element (r / inner) * stride_outer +
 // (r % inner) * stride_inner; its columns are contiguous.  The same split addresses the tokens.

@@ -31,7 +31,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, vocab: int | N
     contiguous, the leading ones may be strided (``logits[:, :-1]`` is not copied).  ``tokens``:
     int64 or int32, the leading shape.  ``vocab``: how many leading columns are real; the others
     (vocabulary padding) take no part and get a zero gradient.  ``top_k``: 0 to 32 alternatives
-    ordered by logit, ties by the lower id; they carry no gradient.
+    ordered by logit, ties by the lower id (of at most 2^21 columns); they carry no gradient.
 
     Rows whose token is ``ignore_index`` are not read: log probability and entropy 0, gradient
     0, alternatives -1 at -inf.  Columns of -inf have probability 0; a row that has no other is
