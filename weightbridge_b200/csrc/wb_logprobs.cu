@@ -26,6 +26,7 @@
 #include "wb_logprobs.h"
 
 #include <cooperative_groups.h>
+#include <cstdlib>
 
 #include "wb_vec.cuh"
 
@@ -83,25 +84,42 @@ __device__ __forceinline__ float rescale(float from, float to, float c2, float& 
   return ex2(shift);
 }
 
-template <int N2>
-__device__ __forceinline__ float tile_max(const F2 (&x)[N2]) {
-  float m = fmaxf(x[0].x, x[0].y);
-  #pragma unroll
-  for (int i = 1; i < N2; ++i) m = fmaxf(m, fmaxf(x[i].x, x[i].y));
-  return m;
+// The largest element of a vector, NaN left out; -inf where there is nothing else.
+template <typename T>
+__device__ __forceinline__ float vec_max(const Vec32& v) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -kInf;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, __uint_as_float(v.w[i]));
+    return m;
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 w[8];
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const T2*>(&v.w[i]);
+    #pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      #pragma unroll
+      for (int i = 0; i < o; ++i) w[i] = __hmax2(w[i], w[i + o]);
+    }
+    return fmaxf(fmaxf(to_f32(w[0].x), to_f32(w[0].y)), -kInf);
+  }
 }
 
-template <int N2>
-__device__ __forceinline__ void accumulate(Stats& t, const F2 (&x)[N2], float top, float c2) {
+__device__ __forceinline__ void raise(Stats& t, float top, float c2) {
   const float m = fmaxf(t.m, top);
   float shift;
   const float f = rescale(t.m, m, c2, shift);
   t.a = mul2(fma2(t.s, F2{shift, shift}, t.a), F2{f, f});
   t.s = mul2(t.s, F2{f, f});
   t.m = m;
+}
+
+template <int N2>
+__device__ __forceinline__ void accumulate(Stats& t, const F2 (&x)[N2], float c2) {
   #pragma unroll
   for (int i = 0; i < N2; ++i) {
-    const F2 z = mul2(add2(x[i], F2{-m, -m}), F2{c2, c2});
+    const F2 z = mul2(add2(x[i], F2{-t.m, -t.m}), F2{c2, c2});
     const F2 e{ex2(z.x), ex2(z.y)};
     t.s = add2(t.s, e);
     t.a = fma2(e, F2{fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)}, t.a);      // 0 * -inf would be NaN
@@ -199,33 +217,42 @@ __device__ __forceinline__ uint32_t tile_before(uint32_t key_j, uint32_t j, uint
   return kKeyShift<T> ? key_j > key_i : key_j + (j < i) > key_i;
 }
 
-// Tiles first, first + step, ... below `end` of a row into this lane's statistics; two at a time,
-// so that the second's load runs under the first's arithmetic.  tops: each tile's largest, as a key.
+// Tiles first, first + step, ... below `end` of a row into this lane's statistics.  Two tiles' loads
+// are always under way: one's vector is refilled as soon as it is unpacked.  tops: each tile's
+// largest, as a key.
 template <typename T, bool TOP>
 __device__ __forceinline__ Stats walk(const T* x, uint32_t vocab, uint32_t mis, uint32_t first, uint32_t step, uint32_t end,
                                       uint32_t base, float c2, uint32_t* tops) {
   constexpr int N = kVecN<T>, kDepth = 2;
   const uint32_t lane = threadIdx.x & 31;
   Stats st;
+  Vec32 raw[kDepth];
+  auto load = [&](int u, uint32_t k) {
+    if (k < end) raw[u] = load_vec(x, vocab, (int32_t)(k * kTile<T> + lane * N - mis));
+  };
+  #pragma unroll
+  for (int u = 0; u < kDepth; ++u) load(u, first + u * step);
+  #pragma unroll 1
   for (uint32_t t = first; t < end; t += kDepth * step) {
-    Vec32 raw[kDepth];
+    float top[kDepth];
     #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
       const uint32_t k = t + u * step;
-      if (k < end) raw[u] = load_vec(x, vocab, (int32_t)(k * kTile<T> + lane * N - mis));
+      top[u] = k < end ? vec_max<T>(raw[u]) : -kInf;
+      if constexpr (TOP) {
+        const uint32_t key = __reduce_max_sync(kFullWarp, order_key(top[u]));
+        if (lane == 0 && k < end) tops[k - base] = tile_key<T>(key, k - base);
+      }
     }
+    raise(st, fmaxf(top[0], top[1]), c2);
     #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
       const uint32_t k = t + u * step;
       if (k >= end) break;
       F2 v[N / 2];
       unpack<T>(raw[u], v);
-      const float top = tile_max(v);
-      accumulate(st, v, top, c2);
-      if constexpr (TOP) {
-        const uint32_t key = __reduce_max_sync(kFullWarp, order_key(fmaxf(top, -kInf)));
-        if (lane == 0) tops[k - base] = tile_key<T>(key, k - base);
-      }
+      load(u, k + kDepth * step);
+      accumulate(st, v, c2);
     }
   }
   return st;
@@ -371,9 +398,7 @@ __device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base
   #pragma unroll
   for (uint32_t s = 0; s < kTopPerWarp; ++s) {
     if (warp + s * kWarps >= picked || j0[s] + N <= 0 || j0[s] >= (int32_t)vocab) continue;      // no column of the row
-    F2 v[N / 2];
-    unpack<T>(raw[s], v);
-    value[s] = order_key(fmaxf(tile_max(v), -kInf)) >> kShift;
+    value[s] = order_key(vec_max<T>(raw[s])) >> kShift;
   }
   // the columns from `from` on of the vectors that `wanted` takes
   auto collect = [&](uint32_t from, auto wanted) {
@@ -415,7 +440,7 @@ __device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base
 
 // A CTA per row, or a cluster of `splits` CTAs.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprobs_row_kernel(const LogprobRows in, const LogprobOut out, const uint32_t splits) {
+__global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const LogprobRows in, const LogprobOut out, const uint32_t splits) {
   extern __shared__ __align__(16) uint32_t tops[];       // TOP: the tiles' maxima, and zeros up to a multiple of four
   __shared__ RowStats warps[kWarps], mine;
   __shared__ std::conditional_t<TOP, TopShared, int> shared;
@@ -580,7 +605,9 @@ cudaError_t launch_rows(const LogprobRows& in, const LogprobOut& out, int sms, c
     return cudaGetLastError();
   }
   uint32_t splits = 1;
-  while (splits < kMaxSplits && (uint64_t)in.rows * splits * 2 <= (uint64_t)sms * 2 && tiles >= splits * 2 * kWarps) splits *= 2;
+  const uint64_t most = (uint64_t)sms * (out.top_k ? 2 : 4);
+  while (splits < kMaxSplits && (uint64_t)in.rows * splits * 2 <= most && tiles >= splits * 2 * kWarps) splits *= 2;
+  if (getenv("WB_SPLITS")) splits = atoi(getenv("WB_SPLITS"));
   const uint32_t per = (tiles + splits - 1) / splits;
   const size_t shared = out.top_k ? 4 * (size_t)per + 16 : 0;
   cudaLaunchConfig_t cfg{};
