@@ -248,25 +248,40 @@ wb::NormTensor norm_tensor(const Tensor& x) {
   return {reinterpret_cast<uint64_t>(x.const_data_ptr()), (uint64_t)x.numel(), float_code(x.scalar_type()), 0};
 }
 
-py::tuple sum_squares(const std::vector<Tensor>& tensors) {
-  if (tensors.empty()) bad("grad_norm: no tensors");
-  const auto dev = tensors[0].device();
+// The norm of the tensors of a dict or a sequence (None entries left out), and the buffer whose
+// first element is the sum of their squares.
+py::tuple sum_squares(const py::object& tensors) {
   std::vector<wb::NormTensor> t;
-  t.reserve(tensors.size());
-  for (const Tensor& x : tensors) {
-    if (!x.is_cuda() || x.device() != dev) bad("grad_norm: all tensors must be CUDA tensors of one device");
+  const Tensor* first = nullptr;
+  auto add = [&](PyObject* o) {
+    if (o == Py_None) return;
+    if (!THPVariable_Check(o)) throw py::type_error("grad_norm: not a tensor");
+    const Tensor& x = THPVariable_Unpack(o);
+    if (!first) first = &x;
+    if (!x.is_cuda() || x.device() != first->device()) bad("grad_norm: all tensors must be CUDA tensors of one device");
     if (!float_code(x.scalar_type())) bad("grad_norm: tensors must be bfloat16, float16 or float32");
     if (!dense(x)) bad("grad_norm: a tensor of shape " + shape_of(x) + " has holes or overlaps in memory");
     if (x.numel()) t.push_back(norm_tensor(x));
+  };
+  if (PyDict_Check(tensors.ptr())) {
+    PyObject *key = nullptr, *value = nullptr;
+    Py_ssize_t pos = 0;
+    t.reserve((size_t)PyDict_Size(tensors.ptr()));
+    while (PyDict_Next(tensors.ptr(), &pos, &key, &value)) add(value);
+  } else {
+    for (const py::handle h : py::reinterpret_borrow<py::sequence>(tensors)) add(h.ptr());
   }
-  const c10::cuda::CUDAGuard guard(dev);
-  const auto f64 = tensors[0].options().dtype(at::kDouble).requires_grad(false);
-  const Tensor partial = partial_sums(t, f64, sm_count(dev.index()));
-  Tensor sum_sq = at::empty({}, f64), norm = at::empty({}, f64.dtype(at::kFloat));
-  check(wb::launch_norm(partial.const_data_ptr<double>(), (uint32_t)partial.numel(), sum_sq.mutable_data_ptr<double>(),
-                        norm.mutable_data_ptr<float>(), c10::cuda::getCurrentCUDAStream()),
-        "grad_norm launch");
-  return py::make_tuple(sum_sq, norm);
+  if (!first) bad("grad_norm: no tensors");
+  const c10::cuda::CUDAGuard guard(first->device());
+  const auto f64 = first->options().dtype(at::kDouble).requires_grad(false);
+  const int sms = sm_count(first->device().index());
+  Tensor buffer = at::empty({1 + (int64_t)wb::partial_sums_size((uint32_t)t.size(), sms)}, f64), norm = at::empty({}, f64.dtype(at::kFloat));
+  double* sum_sq = buffer.mutable_data_ptr<double>();
+  uint32_t n = 0;
+  const auto stream = c10::cuda::getCurrentCUDAStream();
+  check(wb::launch_partial_sums(t.data(), (uint32_t)t.size(), sum_sq + 1, &n, sms, stream), "grad_norm launch");
+  check(wb::launch_norm(sum_sq + 1, n, sum_sq, norm.mutable_data_ptr<float>(), stream), "grad_norm launch");
+  return py::make_tuple(norm, buffer);
 }
 
 // -- AdamW ----------------------------------------------------------------------------------------

@@ -7,12 +7,12 @@
 //   dx_j = ((j == token) g - p_j (g + h (logp_j + H))) / T.
 // A column of -inf has probability 0 and adds nothing to H.  A row without any finite column is
 // empty: log probability -inf, entropy 0, no gradient.  NaN and +inf make the row's results NaN.
-// The difference x - m is taken before the scaling, so rows of the type's lowest value neither
-// overflow nor become empty.  Every sum is held in 32 bits.
+// Rows of the type's lowest value neither overflow nor become empty.  Every sum is held in 32 bits.
 //
-// Forward: one pass.  A warp takes tiles of 1 KiB (32 bytes a lane); every lane keeps its own
-// running (m, S, A) and rescales S and A once per tile, without a branch.  What bounds it is HBM,
-// with the exponentials (16 a clock and SM) close behind: 16-bit logits arrive at 0.7 of their rate.
+// Forward: one pass.  A warp takes tiles of 1 KiB (32 bytes a lane), two loads under way; every lane
+// keeps its own sums.  What bounds it is HBM, with the exponentials (16 a clock and SM: 16-bit
+// logits arrive at 0.7 of their rate) and the instructions around them close behind, so the common
+// path takes five an element: no running maximum, no clamp.  A row that needs them is read again.
 // A CTA of eight warps takes a row; where rows are few, a cluster of CTAs shares one and joins
 // through distributed shared memory (no workspace, no second launch).
 //
@@ -26,7 +26,6 @@
 #include "wb_logprobs.h"
 
 #include <cooperative_groups.h>
-#include <cstdlib>
 
 #include "wb_vec.cuh"
 
@@ -41,6 +40,7 @@ constexpr float kInf = __builtin_huge_valf();
 constexpr float kNaN = __builtin_nanf("");
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
+constexpr float kModerate = 1048576.f;     // 2^20
 constexpr uint32_t kMaxSplits = 8;         // the portable cluster size
 
 template <typename T> constexpr uint32_t kTile = 32u * kVecN<T>;
@@ -72,65 +72,88 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// Running maximum and sums, z in units of ln 2.
+// What z is counted from, in units of ln 2: z = (x - a) c2 - b with c2 = log2(e) / T.  Of an ordinary
+// maximum a = 0 and b is max * c2 rounded to a whole number: z takes one fused operation with one
+// rounding, and shifts between references are exact.  Where max * c2 is too large to be rounded so,
+// a is the maximum itself and b = 0.
+struct Reference {
+  float a, b;
+  __device__ __forceinline__ bool ordinary() const { return a == 0.f; }
+  __device__ __forceinline__ float z(float x, float c2) const { return fmaf(x - a, c2, -b); }
+};
+
+__device__ __forceinline__ Reference reference(float m, float c2) {
+  const float mc = m * c2;
+  const bool ordinary = fabsf(mc) < kModerate;
+  return {ordinary ? 0.f : m, ordinary ? rintf(mc) : 0.f};
+}
+
+// Running maximum and sums.
 struct Stats {
   float m = kLowest;
+  Reference ref{kLowest, 0.f};
   F2 s{0.f, 0.f}, a{0.f, 0.f};
 };
 
-// exp2 of the shift from maximum `from` to `to` >= from; the shift itself, finite, in `shift`
-__device__ __forceinline__ float rescale(float from, float to, float c2, float& shift) {
-  shift = fmaxf((from - to) * c2, -1e30f);
+// exp2 of the shift from one reference to another, of a maximum not below its own; the shift, finite, in `shift`
+__device__ __forceinline__ float rescale(Reference from, Reference to, float c2, float& shift) {
+  shift = fmaxf(fmaf(from.a - to.a, c2, from.b - to.b), -1e30f);
   return ex2(shift);
 }
 
 // The largest element of a vector, NaN left out; -inf where there is nothing else.
-template <typename T>
-__device__ __forceinline__ float vec_max(const Vec32& v) {
-  if constexpr (sizeof(T) == 4) {
-    float m = -kInf;
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, __uint_as_float(v.w[i]));
-    return m;
-  } else {
-    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
-    T2 w[8];
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const T2*>(&v.w[i]);
-    #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-      #pragma unroll
-      for (int i = 0; i < o; ++i) w[i] = __hmax2(w[i], w[i + o]);
-    }
-    return fmaxf(fmaxf(to_f32(w[0].x), to_f32(w[0].y)), -kInf);
-  }
+template <int N2>
+__device__ __forceinline__ float largest(const F2 (&x)[N2]) {
+  float m = -kInf;
+  #pragma unroll
+  for (int i = 0; i < N2; ++i) m = fmaxf(m, fmaxf(x[i].x, x[i].y));
+  return m;
+}
+template <int N2>
+__device__ __forceinline__ float least(const F2 (&x)[N2]) {
+  float m = kInf;
+  #pragma unroll
+  for (int i = 0; i < N2; ++i) m = fminf(m, fminf(x[i].x, x[i].y));
+  return m;
 }
 
 __device__ __forceinline__ void raise(Stats& t, float top, float c2) {
-  const float m = fmaxf(t.m, top);
+  t.m = fmaxf(t.m, top);
+  const Reference to = reference(t.m, c2);
   float shift;
-  const float f = rescale(t.m, m, c2, shift);
+  const float f = rescale(t.ref, to, c2, shift);
   t.a = mul2(fma2(t.s, F2{shift, shift}, t.a), F2{f, f});
   t.s = mul2(t.s, F2{f, f});
-  t.m = m;
+  t.ref = to;
 }
 
-template <int N2>
+// PLAIN: an ordinary reference, and nothing so low that z would not be finite (0 * -inf would be NaN).
+template <bool PLAIN, int N2>
 __device__ __forceinline__ void accumulate(Stats& t, const F2 (&x)[N2], float c2) {
+  const float a = t.ref.a, b = t.ref.b;
   #pragma unroll
   for (int i = 0; i < N2; ++i) {
-    const F2 z = mul2(add2(x[i], F2{-t.m, -t.m}), F2{c2, c2});
+    const F2 z = fma2(PLAIN ? x[i] : add2(x[i], F2{-a, -a}), F2{c2, c2}, F2{-b, -b});
     const F2 e{ex2(z.x), ex2(z.y)};
     t.s = add2(t.s, e);
-    t.a = fma2(e, F2{fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)}, t.a);      // 0 * -inf would be NaN
+    t.a = fma2(e, PLAIN ? z : F2{fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)}, t.a);
   }
+}
+
+// Adds the exponent of S to an ordinary reference (exactly): for sums that have outgrown it.
+__device__ __forceinline__ void lift(Stats& t) {
+  const int e = (int)(__float_as_uint(t.s.x + t.s.y) >> 23) - 127;
+  const float shift = (float)-e, f = __uint_as_float((uint32_t)(127 - e) << 23);
+  t.a = mul2(fma2(t.s, F2{shift, shift}, t.a), F2{f, f});
+  t.s = mul2(t.s, F2{f, f});
+  t.ref.b += (float)e;
 }
 
 struct RowStats { float m, s, a; };
 
 __device__ __forceinline__ RowStats at_max(RowStats t, float m, float c2) {
   float shift;
-  const float f = rescale(t.m, m, c2, shift);
+  const float f = rescale(reference(t.m, c2), reference(m, c2), c2, shift);
   return {m, t.s * f, (t.a + t.s * shift) * f};
 }
 
@@ -162,19 +185,26 @@ __device__ __forceinline__ Vec32 load_vec(const T* x, uint32_t vocab, int32_t j0
   return v;
 }
 
-struct RowResult { float m, ln, entropy; bool empty; };
+struct RowResult {
+  float m, log2_sum, entropy;              // log2_sum: of the exponentials from the reference; +inf: an empty row
+  Reference ref;
+};
 
-__device__ __forceinline__ RowResult finish(RowStats t) {
+__device__ __forceinline__ RowResult finish(RowStats t, float c2) {
+  const bool empty = t.s == 0.f;
   RowResult r;
-  r.empty = t.s == 0.f;
-  r.m = r.empty ? 0.f : t.m;
-  r.ln = r.empty ? kInf : logf(t.s);
-  r.entropy = r.empty ? 0.f : r.ln - kLn2 * t.a / t.s;
+  r.m = empty ? 0.f : t.m;
+  r.ref = reference(r.m, c2);
+  r.log2_sum = empty ? kInf : log2f(t.s);
+  r.entropy = empty ? 0.f : kLn2 * (r.log2_sum - t.a / t.s);
   return r;
 }
 
-__device__ __forceinline__ float logprob(const RowResult& t, float x, float inv_temp) {
-  return t.empty ? -kInf : (x - t.m) * inv_temp - t.ln;
+// Near the type's lowest value z is out of range where the log probability itself may not be; the sum
+// is nothing beside it.
+__device__ __forceinline__ float logprob(const RowResult& t, float x, float c2) {
+  const float z = t.ref.z(x, c2);
+  return z == -kInf && t.log2_sum < kInf ? (x - t.m) * (c2 * kLn2) : kLn2 * (z - t.log2_sum);
 }
 
 // The token's logit, loaded before the row: its latency passes under the row's.
@@ -183,12 +213,13 @@ __device__ __forceinline__ float token_logit(const LogprobRows& in, const T* x, 
   return tok >= 0 && tok < (int64_t)in.vocab ? to_f32(x[tok]) : kNaN;
 }
 
-__device__ __forceinline__ void write_row(const LogprobRows& in, const LogprobOut& out, uint32_t r, int64_t tok, float xt, const RowResult& t) {
-  out.logprobs[r] = tok >= 0 && tok < (int64_t)in.vocab ? logprob(t, xt, in.inv_temp) : kNaN;
+__device__ __forceinline__ void write_row(const LogprobRows& in, const LogprobOut& out, uint32_t r, int64_t tok, float xt, const RowResult& t,
+                                          float c2) {
+  out.logprobs[r] = tok >= 0 && tok < (int64_t)in.vocab ? logprob(t, xt, c2) : kNaN;
   out.entropy[r] = t.entropy;
   if (out.stats) {
     out.stats[2 * (int64_t)r] = t.m;
-    out.stats[2 * (int64_t)r + 1] = t.ln;
+    out.stats[2 * (int64_t)r + 1] = t.log2_sum;
   }
 }
 
@@ -217,67 +248,139 @@ __device__ __forceinline__ uint32_t tile_before(uint32_t key_j, uint32_t j, uint
   return kKeyShift<T> ? key_j > key_i : key_j + (j < i) > key_i;
 }
 
-// Tiles first, first + step, ... below `end` of a row into this lane's statistics.  Two tiles' loads
-// are always under way: one's vector is refilled as soon as it is unpacked.  tops: each tile's
-// largest, as a key.
-template <typename T, bool TOP>
-__device__ __forceinline__ Stats walk(const T* x, uint32_t vocab, uint32_t mis, uint32_t first, uint32_t step, uint32_t end,
-                                      uint32_t base, float c2, uint32_t* tops) {
-  constexpr int N = kVecN<T>, kDepth = 2;
-  const uint32_t lane = threadIdx.x & 31;
-  Stats st;
+// One warp's way through tiles first, first + step, ... below `end` of a row.  Two tiles' loads are
+// always under way: one's vector is refilled as soon as it is unpacked.
+template <typename T>
+struct Walk {
+  static constexpr int N = kVecN<T>, kDepth = 2;
+  const T* x;
+  uint32_t vocab, mis, first, step, end;
   Vec32 raw[kDepth];
-  auto load = [&](int u, uint32_t k) {
-    if (k < end) raw[u] = load_vec(x, vocab, (int32_t)(k * kTile<T> + lane * N - mis));
-  };
-  #pragma unroll
-  for (int u = 0; u < kDepth; ++u) load(u, first + u * step);
-  #pragma unroll 1
-  for (uint32_t t = first; t < end; t += kDepth * step) {
-    float top[kDepth];
+
+  __device__ __forceinline__ void load(int u, uint32_t k) {
+    if (k < end) raw[u] = load_vec(x, vocab, (int32_t)(k * kTile<T> + (threadIdx.x & 31) * N - mis));
+  }
+  // issues the first loads
+  __device__ __forceinline__ void start() {
     #pragma unroll
-    for (int u = 0; u < kDepth; ++u) {
-      const uint32_t k = t + u * step;
-      top[u] = k < end ? vec_max<T>(raw[u]) : -kInf;
-      if constexpr (TOP) {
-        const uint32_t key = __reduce_max_sync(kFullWarp, order_key(top[u]));
-        if (lane == 0 && k < end) tops[k - base] = tile_key<T>(key, k - base);
-      }
+    for (int u = 0; u < kDepth; ++u) load(u, first + u * step);
+  }
+  // This lane's statistics; tops: each tile's largest as a key, counted from tile `base`.
+  template <bool TOP>
+  __device__ __forceinline__ Stats run(float c2, uint32_t base, uint32_t* tops) {
+    Stats st;
+    if (!common<TOP>(st, c2, base, tops)) {
+      start();
+      careful<TOP>(st, c2, base, tops);
     }
-    raise(st, fmaxf(top[0], top[1]), c2);
-    #pragma unroll
-    for (int u = 0; u < kDepth; ++u) {
-      const uint32_t k = t + u * step;
-      if (k >= end) break;
-      F2 v[N / 2];
-      unpack<T>(raw[u], v);
-      load(u, k + kDepth * step);
-      accumulate(st, v, c2);
+    return st;
+  }
+
+ private:
+  template <bool TOP>
+  __device__ __forceinline__ static void keep_top(const F2 (&v)[N / 2], uint32_t tile, uint32_t* tops) {
+    if constexpr (TOP) {
+      const uint32_t key = __reduce_max_sync(kFullWarp, order_key(largest(v)));
+      if ((threadIdx.x & 31) == 0) tops[tile] = tile_key<T>(key, tile);
     }
   }
-  return st;
-}
 
-// Many short rows: a warp takes one after another; the next row's token is under way meanwhile.
+  // Ordinary rows: the first tile's largest gives the reference of the whole walk, which is lifted
+  // where a sum outgrows it, so no maximum is taken of the other tiles.  False (for the whole warp) at
+  // the first sum that is not finite: a masked column (0 * -inf), NaN, or a logit 2^100 times as
+  // probable as the reference.
+  template <bool TOP>
+  __device__ __forceinline__ bool common(Stats& st, float c2, uint32_t base, uint32_t* tops) {
+    if (first >= end) return true;
+    {
+      F2 v[N / 2];
+      unpack<T>(raw[0], v);
+      st.ref = reference(warp_max(largest(v)), c2);
+    }
+    if (!st.ref.ordinary()) return false;
+    const uint32_t full_from = mis ? 1 : 0, full_to = (mis + vocab) / kTile<T>;
+    #pragma unroll 1
+    for (uint32_t t = first; t < end; t += kDepth * step) {
+      #pragma unroll
+      for (int u = 0; u < kDepth; ++u) {
+        const uint32_t k = t + u * step;
+        if (k >= end) break;
+        F2 v[N / 2];
+        unpack<T>(raw[u], v);
+        load(u, k + kDepth * step);
+        keep_top<TOP>(v, k - base, tops);
+        if (k >= full_from && k < full_to) accumulate<true>(st, v, c2);
+        else accumulate<false>(st, v, c2);
+      }
+      const float size = st.a.x + st.a.y;
+      if (__any_sync(kFullWarp, !(fabsf(size) < 1.2676506e30f))) return false;       // 2^100
+      if (size > 65536.f) lift(st);
+    }
+    st.m = st.ref.b / c2;                  // reference(m) gives b again: |b| < 2^21
+    return true;
+  }
+
+  // Any row: the maximum is kept, the sums rescaled to it, and what is too low to count is clamped.
+  template <bool TOP>
+  __device__ __forceinline__ void careful(Stats& st, float c2, uint32_t base, uint32_t* tops) {
+    st = Stats{};
+    #pragma unroll 1
+    for (uint32_t t = first; t < end; t += kDepth * step) {
+      #pragma unroll
+      for (int u = 0; u < kDepth; ++u) {
+        const uint32_t k = t + u * step;
+        if (k >= end) break;
+        F2 v[N / 2];
+        unpack<T>(raw[u], v);
+        load(u, k + kDepth * step);
+        keep_top<TOP>(v, k - base, tops);
+        raise(st, largest(v), c2);
+        accumulate<false>(st, v, c2);
+      }
+    }
+  }
+};
+
+// Many short rows: a warp takes one after another.  The next row's token is under way during a row,
+// and its first tiles while this one's lanes are joined.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) logprobs_warp_kernel(const LogprobRows in, const LogprobOut out) {
   const uint32_t warps = gridDim.x * kWarps, lane = threadIdx.x & 31;
   const float c2 = in.inv_temp * kLog2e;
-  uint32_t r = blockIdx.x * kWarps + threadIdx.x / 32;
-  int64_t next = r < in.rows ? token_of(in, r) : 0;
-  for (; r < in.rows; r += warps) {
-    const int64_t tok = next;
-    if (in.rows - r > warps) next = token_of(in, r + warps);
-    if (tok == in.ignore_index) {
+  uint32_t next = blockIdx.x * kWarps + threadIdx.x / 32;          // the row that `ahead` is the token of
+  int64_t ahead = next < in.rows ? token_of(in, next) : 0;
+  uint32_t r = 0;
+  int64_t tok = 0;
+  float xt = 0.f;
+  Walk<T> w;
+  auto open = [&] {                                                // the next row that is not ignored
+    for (; next < in.rows; next += warps) {
+      r = next;
+      tok = ahead;
+      if (in.rows - next > warps) ahead = token_of(in, next + warps);
+      if (tok != in.ignore_index) {
+        w.x = row_ptr<T>(in, r);
+        w.mis = misaligned(w.x);
+        w.vocab = in.vocab;
+        w.first = 0, w.step = 1, w.end = (w.mis + in.vocab + kTile<T> - 1) / kTile<T>;
+        w.start();
+        xt = token_logit(in, w.x, tok);
+        next += warps;
+        return true;
+      }
       if (lane == 0) write_ignored(out, r);
-      continue;
     }
-    const T* x = row_ptr<T>(in, r);
-    const float xt = token_logit(in, x, tok);
-    const uint32_t mis = misaligned(x), tiles = (mis + in.vocab + kTile<T> - 1) / kTile<T>;
-    const Stats st = walk<T, false>(x, in.vocab, mis, 0, 1, tiles, 0, c2, nullptr);
+    return false;
+  };
+  bool more = open();
+  while (more) {
+    const Stats st = w.template run<false>(c2, 0, nullptr);
+    const uint32_t row = r;
+    const int64_t row_tok = tok;
+    const float row_xt = xt;
+    more = open();
     const RowStats t = warp_join({st.m, st.s.x + st.s.y, st.a.x + st.a.y}, c2);
-    if (lane == 0) write_row(in, out, r, tok, xt, finish(t));
+    if (lane == 0) write_row(in, out, row, row_tok, row_xt, finish(t, c2), c2);
   }
 }
 
@@ -339,14 +442,13 @@ __device__ __forceinline__ void rank_candidates(const uint64_t* c, uint32_t n, u
   }
 }
 
-// The k first columns of tiles [base, base + n), in order, into sh.out.  top: the largest logit of
-// these tiles; tops: each tile's, as a key.
+// The k first columns of tiles [base, base + n), in order, into sh.out.  tops: each tile's largest.
 template <typename T>
-__device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base, uint32_t n, uint32_t k, float top, const uint32_t* tops,
+__device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base, uint32_t n, uint32_t k, const uint32_t* tops,
                          TopShared& sh) {
   constexpr int N = kVecN<T>, kShift = kKeyShift<T>;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const uint32_t high = order_key(top) >> kShift;
+  constexpr uint32_t high = 0xffffffffu >> kShift;
   uint32_t turn = 0;
   const bool counted = n <= 2 * kThreads;
   if (threadIdx.x == 0) sh.n_picked = sh.n_candidates = 0, sh.least = 1;
@@ -398,7 +500,9 @@ __device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base
   #pragma unroll
   for (uint32_t s = 0; s < kTopPerWarp; ++s) {
     if (warp + s * kWarps >= picked || j0[s] + N <= 0 || j0[s] >= (int32_t)vocab) continue;      // no column of the row
-    value[s] = order_key(vec_max<T>(raw[s])) >> kShift;
+    F2 v[N / 2];
+    unpack<T>(raw[s], v);
+    value[s] = order_key(largest(v)) >> kShift;
   }
   // the columns from `from` on of the vectors that `wanted` takes
   auto collect = [&](uint32_t from, auto wanted) {
@@ -458,19 +562,21 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const Logprob
     return;
   }
   const T* x = row_ptr<T>(in, r);
-  const float xt = token_logit(in, x, tok);
   const float c2 = in.inv_temp * kLog2e;
   const uint32_t mis = misaligned(x), tiles = (mis + in.vocab + kTile<T> - 1) / kTile<T>;
   const uint32_t per = (tiles + splits - 1) / splits;
   const uint32_t begin = min(split * per, tiles), end = min(begin + per, tiles);
   if (TOP && threadIdx.x < 4) tops[(end - begin) + threadIdx.x] = 0;
-  const Stats st = walk<T, TOP>(x, in.vocab, mis, begin + warp, kWarps, end, begin, c2, tops);
+  Walk<T> walk{x, in.vocab, mis, begin + warp, kWarps, end, {}};
+  walk.start();
+  const float xt = token_logit(in, x, tok);
+  const Stats st = walk.template run<TOP>(c2, begin, tops);
   const RowStats w = warp_join({st.m, st.s.x + st.s.y, st.a.x + st.a.y}, c2);
   if (lane == 0) warps[warp] = w;
   __syncthreads();
   // every warp joins the eight: the same operations, the same bits
   RowStats all = warp_join(lane < kWarps ? warps[lane] : RowStats{kLowest, 0.f, 0.f}, c2);
-  if constexpr (TOP) find_top(x, in.vocab, mis, begin, end - begin, (uint32_t)out.top_k, all.m, tops, shared);
+  if constexpr (TOP) find_top(x, in.vocab, mis, begin, end - begin, (uint32_t)out.top_k, tops, shared);
   if (splits > 1) {
     cg::cluster_group cl = cg::this_cluster();
     if (threadIdx.x == 0) mine = all;
@@ -495,12 +601,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const Logprob
     cl.sync();                             // the others' shared memory stays until it has been read
   }
   if (split == 0 && warp == 0) {
-    const RowResult t = finish(all);
-    if (lane == 0) write_row(in, out, r, tok, xt, t);
+    const RowResult t = finish(all, c2);
+    if (lane == 0) write_row(in, out, r, tok, xt, t, c2);
     if constexpr (TOP) {
       if (lane < (uint32_t)out.top_k) {
         const uint64_t c = shared.out[lane];
-        out.top_logprobs[(int64_t)r * out.top_k + lane] = logprob(t, key_value((uint32_t)(c >> 32)), in.inv_temp);
+        out.top_logprobs[(int64_t)r * out.top_k + lane] = logprob(t, key_value((uint32_t)(c >> 32)), c2);
         out.top_ids[(int64_t)r * out.top_k + lane] = (int64_t)(uint32_t)~(uint32_t)c;
       }
     }
@@ -515,7 +621,7 @@ constexpr uint32_t kGradTiles = 16;        // tiles of one warp's work: 16 KiB r
 // otherwise (views whose rows are not multiples of 32 bytes), and at the ends of a row, lanes take
 // single elements side by side instead of vectors.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_grad_kernel(const LogprobRows in, const LogprobGrad g, const uint32_t segs,
+__global__ void __launch_bounds__(kThreads, 4) logprobs_grad_kernel(const LogprobRows in, const LogprobGrad g, const uint32_t segs,
                                                                  const uint64_t units) {
   constexpr int N = kVecN<T>;
   const uint64_t unit = (uint64_t)blockIdx.x * kWarps + threadIdx.x / 32;
@@ -525,18 +631,25 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad_kernel(const LogprobRo
   const T* x = row_ptr<T>(in, r);
   T* d = reinterpret_cast<T*>(g.grad) + (int64_t)r * g.cols;
   const uint32_t mis = misaligned(d);
-  const float m = g.stats[2 * (int64_t)r], ln = g.stats[2 * (int64_t)r + 1], h = g.entropy[r];
+  const float c2 = in.inv_temp * kLog2e, m = g.stats[2 * (int64_t)r], log2_sum = g.stats[2 * (int64_t)r + 1], h = g.entropy[r];
   float glp = g.g_logprobs ? g.g_logprobs[r * g.g_logprobs_stride] : 0.f;
   float gh = g.g_entropy ? g.g_entropy[r * g.g_entropy_stride] : 0.f;
-  const bool dead = tok == in.ignore_index || ln == kInf;
+  const bool dead = tok == in.ignore_index || log2_sum == kInf;
   if (dead) glp = gh = 0.f;
   else if (tok < 0 || tok >= (int64_t)in.vocab) glp = kNaN;
-  // dx = p (a + b log2 p), and onehot at the token
-  const float c2 = in.inv_temp * kLog2e, l2 = ln * kLog2e;
-  const float a = -in.inv_temp * (glp + gh * h), b = -in.inv_temp * gh * kLn2, onehot = glp * in.inv_temp;
-  auto grad2 = [&](F2 v) {
-    const F2 z = fma2(add2(v, F2{-m, -m}), F2{c2, c2}, F2{-l2, -l2});
-    return mul2(F2{ex2(z.x), ex2(z.y)}, fma2(F2{b, b}, F2{fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)}, F2{a, a}));
+  // log2 p = z - f, z counted from a whole number more and f the rest of log2_sum: with
+  // dx = p (c + d log2 p) = 2^z 2^-f (c - d f + d z) the constants take the rest in
+  const Reference ref = reference(m, c2);
+  const float whole = dead ? 0.f : rintf(log2_sum), f = dead ? 0.f : log2_sum - whole, k = ex2(-f);
+  const float d1 = -k * in.inv_temp * gh * kLn2, c1 = -k * in.inv_temp * (glp + gh * h) - d1 * f, onehot = glp * in.inv_temp;
+  const float a = ref.a, b = ref.b + whole, lowest = -kModerate / c2;
+  auto plain2 = [&](F2 v) {
+    const F2 z = fma2(v, F2{c2, c2}, F2{-b, -b});
+    return mul2(F2{ex2(z.x), ex2(z.y)}, fma2(F2{d1, d1}, z, F2{c1, c1}));
+  };
+  auto safe2 = [&](F2 v) {                               // as in accumulate()
+    const F2 z = fma2(add2(v, F2{-a, -a}), F2{c2, c2}, F2{-b, -b});
+    return mul2(F2{ex2(z.x), ex2(z.y)}, fma2(F2{d1, d1}, F2{fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)}, F2{c1, c1}));
   };
   const bool vectors = misaligned(x) == mis;
   const uint32_t tiles = (mis + g.cols + kTile<T> - 1) / kTile<T>;
@@ -552,8 +665,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad_kernel(const LogprobRo
         for (int i = 0; i < N / 2; ++i) v[i] = {0.f, 0.f};
       } else {
         unpack<T>(load32(x + j0), v);
-        #pragma unroll
-        for (int i = 0; i < N / 2; ++i) v[i] = grad2(v[i]);
+        if (ref.ordinary() && least(v) > lowest) {
+          #pragma unroll
+          for (int i = 0; i < N / 2; ++i) v[i] = plain2(v[i]);
+        } else {
+          #pragma unroll
+          for (int i = 0; i < N / 2; ++i) v[i] = safe2(v[i]);
+        }
         if (tok >= j0 && tok < j0 + N) {
           #pragma unroll
           for (int i = 0; i < N / 2; ++i) {
@@ -566,17 +684,20 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad_kernel(const LogprobRo
     } else {
       // a lane that passes the row's ends: its own elements; rows that lie otherwise: side by side
       const int32_t first = vectors ? j0 : tile0 + (int32_t)lane, step = vectors ? 1 : 32;
-      float v[N];
-      #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int32_t j = first + e * step;
-        v[e] = !dead && j >= 0 && j < (int32_t)in.vocab ? to_f32(x[j]) : -kInf;
-      }
-      #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int32_t j = first + e * step;
-        const float y = j < (int32_t)in.vocab && !dead ? grad2({v[e], v[e]}).x + (j == tok ? onehot : 0.f) : 0.f;
-        if (j >= 0 && j < (int32_t)g.cols) d[j] = from_f32<T>(y);
+      #pragma unroll 1
+      for (int e = 0; e < N; e += 8) {
+        float v[8];
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int32_t j = first + (e + i) * step;
+          v[i] = !dead && j >= 0 && j < (int32_t)in.vocab ? to_f32(x[j]) : -kInf;
+        }
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int32_t j = first + (e + i) * step;
+          const float y = j < (int32_t)in.vocab && !dead ? safe2({v[i], v[i]}).x + (j == tok ? onehot : 0.f) : 0.f;
+          if (j >= 0 && j < (int32_t)g.cols) d[j] = from_f32<T>(y);
+        }
       }
     }
   }
@@ -597,17 +718,21 @@ bool ok(const LogprobRows& in) { return in.rows < 0x7fffffffu && in.vocab >= 1 &
 template <typename T>
 cudaError_t launch_rows(const LogprobRows& in, const LogprobOut& out, int sms, cudaStream_t stream) {
   const uint32_t tiles = (in.vocab + kTile<T> - 1) / kTile<T> + 1;
-  // A warp a row: no barrier, no second join.  For rows of up to four tiles, of which a CTA's eight
-  // warps would find no two; and for up to 32 where the rows fill half of the GPU's warps.
-  if (!out.top_k && (tiles <= 5 || (tiles <= 33 && in.rows >= (uint32_t)sms * 16))) {
+  // A warp a row where the rows alone fill the GPU: no barrier, no second join.  The more tiles a row
+  // has, the more rows it takes until a CTA's eight warps a row lose (bf16, warp against CTA: 1000 x
+  // 4000 6.5 and 6.7 us, 2000 x 8000 12.0 and 13.7, 4096 x 16000 31.9 and 36.3, 20000 x 32000 231
+  // and 249; the other way 500 x 4000 4.9 and 3.9, 2000 x 32000 36.3 and 30.1, 4096 x 128256 209 and 175).
+  if (!out.top_k && tiles <= 65 && (uint64_t)tiles * sms * 2 <= (uint64_t)in.rows * 3) {
     const uint32_t cap = (uint32_t)sms * 4, grid = (in.rows + kWarps - 1) / kWarps;
     logprobs_warp_kernel<T><<<grid < cap ? grid : cap, kThreads, 0, stream>>>(in, out);
     return cudaGetLastError();
   }
+  // CTAs of a row: until two (with alternatives, whose search every CTA repeats) or four of the four
+  // that an SM holds are taken, and every warp keeps two tiles (bf16, 64 x 151936: 1 CTA 23 us, 2: 15,
+  // 4: 11.1, 8: 10.4; 512 rows: 1 CTA 41, 2: 45).
   uint32_t splits = 1;
   const uint64_t most = (uint64_t)sms * (out.top_k ? 2 : 4);
   while (splits < kMaxSplits && (uint64_t)in.rows * splits * 2 <= most && tiles >= splits * 2 * kWarps) splits *= 2;
-  if (getenv("WB_SPLITS")) splits = atoi(getenv("WB_SPLITS"));
   const uint32_t per = (tiles + splits - 1) / splits;
   const size_t shared = out.top_k ? 4 * (size_t)per + 16 : 0;
   cudaLaunchConfig_t cfg{};

@@ -29,7 +29,7 @@ struct LogprobRows {
 struct LogprobOut {
   float* logprobs;             // [rows]
   float* entropy;              // [rows]
-  float* stats;                // [rows, 2]: max logit and ln sum (+inf: an empty row), or null
+  float* stats;                // [rows, 2]: max logit and log2 of the sum (+inf: an empty row), or null
   float* top_logprobs;         // [rows, top_k] or null
   int64_t* top_ids;
   int top_k;                   // 0 .. kLogprobMaxTop

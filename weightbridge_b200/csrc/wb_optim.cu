@@ -607,7 +607,8 @@ cudaError_t launch_partial_sums(NormTensor* t, uint32_t n, double* partial, uint
   for (uint32_t first = 0; first < n; first += kNormTensorsPerLaunch) {
     const uint32_t k = n - first < kNormTensorsPerLaunch ? n - first : kNormTensorsPerLaunch;
     *n_partial += k <= 128 ? partial_sums_launch<128>(t + first, k, partial + *n_partial, sms, stream)
-                           : partial_sums_launch<kNormTensorsPerLaunch>(t + first, k, partial + *n_partial, sms, stream);
+                  : k <= 512 ? partial_sums_launch<512>(t + first, k, partial + *n_partial, sms, stream)
+                             : partial_sums_launch<kNormTensorsPerLaunch>(t + first, k, partial + *n_partial, sms, stream);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }

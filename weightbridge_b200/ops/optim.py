@@ -21,10 +21,12 @@ def grad_norm(tensors: Mapping[str, torch.Tensor] | Iterable[torch.Tensor], grou
     which the squares are summed; a tensor that several of its ranks hold counts once per rank.
     Squares are formed in 32 bits: a gradient above 1.8e19 makes the norm infinite.
     """
-    ts = [t for t in (tensors.values() if isinstance(tensors, Mapping) else tensors) if t is not None]
-    sum_sq, norm = ext().sum_squares(ts)
+    if not isinstance(tensors, (dict, list, tuple)):
+        tensors = dict(tensors) if isinstance(tensors, Mapping) else list(tensors)
+    norm, buffer = ext().sum_squares(tensors)
     if group is None:
         return norm
+    sum_sq = buffer[0]
     torch.distributed.all_reduce(sum_sq, group=group)
     return sum_sq.sqrt().float()
 
