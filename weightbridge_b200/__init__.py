@@ -4,7 +4,8 @@ Public API (the names of the reference package ``wbridge``, ``wbridge/__init__.p
 ``WeightSender``, ``WeightReceiver``, ``WeightReceiverController``, ``WeightData``,
 ``dtype_str_to_torch``, ``dtype_to_str``; plus ``TransferConfig`` and the layout adapters
 ``MegatronLayout`` / ``FSDPLayout`` (trainers) and ``SGLangLayout`` (rollout), and the operators
-of an RL step beside the sync: ``token_logprobs``, ``AdamW`` and ``grad_norm``.
+of an RL step beside the sync: ``token_logprobs`` (and ``policy_gap``, which checks a sync by them),
+``AdamW`` and ``grad_norm``.
 """
 from .core.shard import (WeightData, check_shard_compatibility, original_total_numel,
                          shards_iterator)
@@ -29,6 +30,9 @@ def __getattr__(name):
     if name in ("token_logprobs", "TokenLogprobs"):
         from .ops import logprobs
         return getattr(logprobs, name)
+    if name in ("policy_gap", "PolicyGap"):
+        from .control import policy
+        return getattr(policy, name)
     if name in ("AdamW", "grad_norm"):
         from .ops import optim
         return getattr(optim, name)
@@ -39,6 +43,6 @@ __all__ = [
     "WeightData", "WeightSender", "WeightReceiver", "WeightReceiverController", "TransferConfig",
     "check_shard_compatibility", "shards_iterator", "original_total_numel", "dtype_str_to_torch",
     "dtype_to_str", "MegatronLayout", "FSDPLayout", "HFLayout", "SGLangLayout", "VLLMLayout",
-    "token_logprobs", "TokenLogprobs", "AdamW", "grad_norm",
+    "token_logprobs", "TokenLogprobs", "policy_gap", "PolicyGap", "AdamW", "grad_norm",
 ]
 __version__ = "0.1.0"

@@ -47,6 +47,7 @@ from ..core.plancache import PlanCache, plan_key, relative_binding
 from ..core.shard import WeightData, covered_numel, shard_numel
 from ..utils.config import WIRE_MODES, TransferConfig, normalize_mode
 from .assign import assign_sources, restrict
+from .policy import PolicyGap, policy_gap
 from ..utils.trace import nvtx_range
 from .protocol import PROTOCOL_VERSION, gpu_id
 from .session import Janitor, PeerError, Session, SessionTimeout, local_address
@@ -152,6 +153,8 @@ class WeightSender:
         self.targets: dict[int, list[str]] = {}
         self.overlaps: dict[int, WeightData] = {}
         self.history: list[SyncStats] = []
+        self.version: int | None = None              # version tag of the last sync that completed
+        self.last_gap: PolicyGap | None = None       # of the last check_policy
         self._program = None
         self._program_key = None
         self._routes: list[tuple[list[int], int]] = []   # (receivers one store reaches, bytes) of the program
@@ -1053,11 +1056,32 @@ class WeightSender:
         else:
             stream.wait_stream(after if after is not None else torch.cuda.current_stream(device))
 
+    def check_policy(self, logits: torch.Tensor, tokens: torch.Tensor, rollout_logprobs: torch.Tensor, *,
+                     version: int | None = None, tolerance: float | None = None, vocab: int | None = None,
+                     temperature: float = 1.0, ignore_index: int = -100) -> PolicyGap:
+        """Whether the rollout serves the policy that was sent: the log probabilities it returned
+        with its sampled ``tokens`` against this trainer's, from ``logits`` computed with the weights
+        of the last sync (``policy_gap`` has the arguments; with padded positions, tokens of
+        ``ignore_index``).  ``version``: the weights version the rollout sampled with; ``ValueError``
+        where the last completed sync carried another.  ``tolerance``: ``TransferError`` where the
+        mean difference is above it.  This rank's tokens only; no other rank takes part."""
+        if version is not None and version != self.version:
+            raise ValueError(f"the rollout sampled with weights version {version}, the last sync carried {self.version}")
+        gap = policy_gap(logits, tokens, rollout_logprobs, vocab=vocab, temperature=temperature, ignore_index=ignore_index)
+        gap.version = self.version
+        self.last_gap = gap
+        if tolerance is not None and not gap.within(tolerance):
+            raise TransferError(f"the rollout does not serve the trainer's policy: its log probabilities are off by {gap.mean_abs:.3g} "
+                                f"on average (at most {gap.max_abs:.3g}) over {gap.tokens} tokens, above {tolerance:.3g}")
+        return gap
+
     def summary(self, last: int = 100) -> dict:
         """Median and 90th percentile of the last ``last`` syncs' host time, device time, wait
-        for the workers and GB/s (``SyncStats``), for periodic logging."""
+        for the workers and GB/s (``SyncStats``), for periodic logging; the last policy check."""
         hist = self.history[-last:]
         out: dict = {"syncs": len(hist)}
+        if self.last_gap is not None:
+            out["policy_gap"] = dict(self.last_gap.__dict__)
         if not hist:
             return out
         for f in ("host_ms", "device_ms", "wait_ready_ms", "exchange_ms", "gbs"):
@@ -1105,6 +1129,7 @@ class WeightSender:
         elif self._writes_nothing:        # rank 0 arms every worker even when it sends nothing itself
             self._arm_and_check(epoch)
         self.epoch = epoch
+        self.version = version if version >= 0 else None
         st.marks["end"] = time.perf_counter()
         st.host_ms = (st.marks["end"] - t0) * 1e3
         self.history.append(st)

@@ -18,6 +18,10 @@ peer-push / peer-pull / peer-quant (two GPUs, one process, peer access enabled):
          GPU 0 into GPU 1; bandwidth counts the bytes that cross NVLink.
 peer-peak: copy engine, push kernel and pull kernel GPU 0 -> GPU 1, best of --iters each;
          the largest is the measured peer peak (--out writes it as JSON).
+logprobs: [rows, 128256] bf16 logits scored (no gradient); logprobs-grad: the same with the
+         gradient of the logits (--rows);
+adamw / adamw8: one clipped step over bf16 matrices of 4096 x 4096 (--gbytes: their bytes), states in
+         32 bits with fp32 master weights / in 8 bits; norm: the gradient norm alone.
 Reports device time per launch (CUDA events, after warm-up) and achieved bandwidth against
 the measured copy peak in MEASURED_PEAKS.json when present.
 """
@@ -293,12 +297,52 @@ def mc_peak(gbytes: float, iters: int, warmup: int, item_bytes: int, members: in
     return out
 
 
+def learn(case: str, gbytes: float, rows: int, dev, iters: int, warmup: int) -> dict:
+    """One of the operators beside the sync; traffic: what it has to move (each input once, each
+    output once; the clipped step reads its gradients twice, once for the norm)."""
+    from .logprobs import token_logprobs
+    from .optim import AdamW, grad_norm
+    if case.startswith("logprobs"):
+        vocab = 128256
+        x = torch.empty(rows, vocab, device=dev, dtype=torch.bfloat16).normal_(0, 2.5)
+        t = torch.randint(0, vocab, (rows,), device=dev)
+        if case == "logprobs":
+            call, traffic = (lambda: token_logprobs(x, t)), x.nbytes
+        else:
+            x.requires_grad_()
+            g = torch.ones(rows, device=dev)
+
+            def call():
+                out = token_logprobs(x, t)
+                torch.autograd.grad((out.logprobs, out.entropy), x, (g, g))
+            traffic = 3 * x.nbytes
+    else:
+        n = max(1, int(gbytes * (1 << 30)) // (2 * 4096 * 4096))
+        params = {f"w{i}": torch.empty(4096, 4096, device=dev, dtype=torch.bfloat16).normal_(0, 0.02) for i in range(n)}
+        grads = {k: torch.empty_like(p).normal_(0, 1e-3) for k, p in params.items()}
+        each = n * 4096 * 4096
+        if case == "norm":
+            call, traffic = (lambda: grad_norm(grads)), 2 * each
+        else:
+            opt = AdamW(params, states="fp8" if case == "adamw8" else "fp32", master=case == "adamw")
+            call = lambda: opt.step(grads, max_norm=1.0)  # noqa: E731
+            traffic = each * (2 + 2 + 2 + (8 + 16 if case == "adamw" else 2 + 4 + 16 / 128))
+    ms = _time_ms(call, iters, warmup, torch.cuda.current_stream(dev))
+    gbs, peak = traffic / (ms / 1e3) / 1e9, _peak_gbs()
+    return {"case": case, "ms": round(ms, 4), "traffic_bytes": int(traffic), "gbs": round(gbs, 1),
+            "frac_of_measured": round(gbs / peak, 3) if peak else None}
+
+
+LEARN_CASES = ("logprobs", "logprobs-grad", "adamw", "adamw8", "norm")
+
+
 def main(argv=None):
     p = argparse.ArgumentParser()
     p.add_argument("--case", default="copy",
                    choices=["copy", "strided", "transpose", "quant", "mixed", "split", "peer-push", "peer-pull", "peer-quant",
-                            "peer-peak", "mc-peak"])
+                            "peer-peak", "mc-peak", *LEARN_CASES])
     p.add_argument("--gbytes", type=float, default=1.0)
+    p.add_argument("--rows", type=int, default=4096, help="logprobs: rows of logits")
     p.add_argument("--mode", type=int, default=-1)
     p.add_argument("--piece", type=int, default=16384)
     p.add_argument("--grid", type=int, default=0)
@@ -324,6 +368,9 @@ def main(argv=None):
         return
     dev = torch.device("cuda", 1 if a.case == "peer-pull" else 0)   # pull: the kernel runs on the reader
     torch.cuda.set_device(dev)
+    if a.case in LEARN_CASES:
+        print(json.dumps(learn(a.case, a.gbytes, a.rows, dev, a.iters, a.warmup)))
+        return
     tables, keep, traffic = build(a.case, a.gbytes, dev, a.item_bytes)
     prog = TransferProgram(tables, dev, [], LaunchConfig(mode=a.mode, piece_bytes=a.piece, grid=a.grid or None))
     if prog.n_pieces:          # split pieces: a real amax pass first, timed separately
