@@ -91,8 +91,9 @@ def _check_grad(d, g1, g2, lp, h, logp, p, keep, tokens, vocab, temperature, tol
     want = (a * (one - p) - b * p * (fl + h[:, None])) / temperature
     size = p * (a.abs() + b.abs() * (fl.abs() + h[:, None])) + one * a.abs()
     tol = size * (U * (16 + 8 * fl.abs()) + tol_lp[:, None]) + p * b.abs() * (tol_lp + tol_h)[:, None]
-    # a probability below the normal numbers of fp32 (2^-126) may be taken as 0
-    tol = tol + 2.0 ** -126 * (a.abs() + b.abs() * (fl.abs() + h[:, None]))
+    # p = 2^z 2^-f with |f| <= 1/2, and a 2^z below the normal numbers of fp32 (2^-126) may be taken as
+    # 0: so may a probability below 2^-125.5
+    tol = tol + 2.0 ** -125.5 * (a.abs() + b.abs() * (fl.abs() + h[:, None]))
     half = torch.finfo(d.dtype).eps / 2
     tol = tol / temperature * 1.01 + half * want.abs() * 1.01 + torch.finfo(d.dtype).tiny * torch.finfo(d.dtype).eps
     assert torch.equal(d[:, vocab:], torch.zeros_like(d[:, vocab:]))
@@ -278,6 +279,36 @@ def test_partial_gradients_none_and_second_derivative():
 
 
 @gpu
+@pytest.mark.parametrize("temperature", [1e-30, 1e-6, 1e-2, 50.0, 1e6, 1e30])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_temperatures(temperature, dtype):
+    """From one-hot rows to uniform ones; z is finite or -inf in between, and exact ties stay ties."""
+    x, t = _inputs(6, 3001, dtype, seed=11)
+    t[0] = int(x[0].argmax())
+    x[1, 5] = x[1, 7] = 30.0                                     # two largest
+    t[1] = 7
+    _check(x, t, temperature=temperature, top_k=5, grad=temperature >= 1e-2)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [1500, 40000])
+def test_rows_that_outgrow_their_beginning(dtype, vocab):
+    """The largest logits come last, a little or far above the first ones (2^20 to 2^200 times as
+    probable), in steps, and below them."""
+    x, t = _inputs(8, vocab, dtype, seed=12, std=1.0)
+    for row, up in enumerate((15.0, 40.0, 60.0, 80.0, 140.0)):
+        x[row, -3:] += up
+    x[5] += torch.linspace(-60, 60, vocab, device="cuda").to(dtype)
+    x[6] += torch.linspace(60, -60, vocab, device="cuda").to(dtype)
+    x[7, :vocab // 2] -= 200.0
+    t[::2] = vocab - 2
+    _check(x, t, top_k=10)
+    x *= 1000.0                                                 # large logits, far apart
+    _check(x, t, top_k=10, grad=False)
+
+
+@gpu
 def test_no_rows():
     x = torch.randn(0, 64, device="cuda", requires_grad=True)
     out = token_logprobs(x, torch.zeros(0, dtype=torch.long, device="cuda"), top_k=3)
@@ -370,9 +401,10 @@ def test_refusals():
     refused("top_k must be between 0 and 3", vocab=3, top_k=4)
     refused("at most 2097152 columns", torch.empty(1, 2 ** 21 + 1, dtype=torch.float16), torch.zeros(1, dtype=torch.long), top_k=1)
     refused("2\\^30 columns", torch.empty(1, dtype=torch.float16).expand(1, 2 ** 30 + 1), torch.zeros(1, dtype=torch.long))
-    for v in (0.0, -1.0, math.nan, math.inf, 1e-60):
+    for v in (0.0, -1.0, math.nan, math.inf, 1e-60, 1e60):
         refused("temperature", temperature=v)
     refused("contiguous", torch.randn(10, 4).t())
     refused("vocab must be", torch.randn(4, 0))
+    refused("sparse", x.to_sparse())
     with pytest.raises(TypeError):
         token_logprobs([[1.0]], t)

@@ -338,6 +338,10 @@ def test_refusals_on_the_gpu():
             opt.step({"a": g}, max_norm=bad)
     with pytest.raises(ValueError, match="lr"):
         opt.step({"a": g}, lr=-1.0)
+    with pytest.raises(ValueError, match="sparse"):
+        opt.step({"a": g.to_sparse()})
+    with pytest.raises(ValueError, match="sparse"):
+        grad_norm([g.to_sparse()])
     with pytest.raises(ValueError, match="one value per element"):
         opt.slices(torch.zeros(3))
     for tensors, match in (([], "no tensors"), ([g.long()], "bfloat16"), ([g, g.cpu()], "device"), ([g[:, :3]], "holes")):
@@ -372,9 +376,36 @@ def test_refusals_without_a_gpu():
     with pytest.raises(ValueError, match="CUDA"):
         grad_norm(p)
     for kw, match in ((dict(states="int8"), "states"), (dict(betas=(1.0, 0.9)), "betas"), (dict(betas=(0.9, -0.1)), "betas"),
-                      (dict(eps=0.0), "eps"), (dict(weight_decay=-1.0), "eps"), (dict(lr=-1.0), "lr"), (dict(no_decay=["b"]), "no_decay")):
+                      (dict(eps=0.0), "eps"), (dict(eps=1e-40), "eps"), (dict(lr=math.inf), "lr"), (dict(weight_decay=-1.0), "eps"), (dict(lr=-1.0), "lr"), (dict(no_decay=["b"]), "no_decay")):
         with pytest.raises(ValueError, match=match):
             AdamW(p, **kw)
+
+
+@gpu
+def test_fsdp_parameters_by_their_local_tensors():
+    """DTensors are refused; the views that convert_to_wb makes of them are the local tensors."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import DeviceMesh
+    from torch.distributed.tensor import Shard, distribute_tensor
+    from weightbridge_b200.parallel.fsdp import convert_to_wb
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        mesh = DeviceMesh("cuda", [0])
+        p = distribute_tensor(torch.ones(64, 8, device="cuda"), mesh, [Shard(0)])
+        g = distribute_tensor(torch.full((64, 8), 2.0, device="cuda"), mesh, [Shard(0)])
+        with pytest.raises(ValueError, match="DTensor"):
+            AdamW({"p": p})
+        with pytest.raises(ValueError, match="DTensor"):
+            grad_norm({"p": g})
+        _, views = convert_to_wb({"p": p})
+        opt = AdamW(views, lr=0.5, weight_decay=0.0)
+        with pytest.raises(ValueError, match="DTensor"):
+            opt.step({"p": g})
+        norm = opt.step({"p": g.to_local()}, max_norm=1e9)
+        assert abs(float(norm) - 2.0 * math.sqrt(512)) < 1e-4
+        assert float((p.to_local() - 0.5).abs().max()) < 1e-6       # the first step is lr along the gradient's sign
+    finally:
+        dist.destroy_process_group()
 
 
 def _rank(rank, port, out):

@@ -48,6 +48,10 @@ std::string shape_of(const Tensor& t) {
   return s + "]";
 }
 
+// Wrappers of other tensors (DTensor and the like) have no memory of their own.
+bool wrapped(const Tensor& t) { return t.layout() != at::kStrided || t.key_set().has(c10::DispatchKey::Python); }
+constexpr const char* kWrapped = " is a sparse tensor or a wrapper (DTensor): give the plain local tensor (to_local())";
+
 int sm_count(int device) {
   static std::array<int, 64> known{};          // one attribute query per device; the value never changes
   int v = device < 64 ? known[device] : 0;
@@ -204,6 +208,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 
 py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::optional<int64_t>& columns, double temperature,
                          int64_t top_k, int64_t ignore_index) {
+  if (wrapped(logits) || wrapped(tokens)) bad(std::string("token_logprobs: an argument") + kWrapped);
   if (logits.dim() < 1) bad("token_logprobs: logits need a vocabulary dimension");
   const int64_t cols = logits.size(-1), vocab = columns.value_or(cols);
   if (!float_code(logits.scalar_type())) bad("token_logprobs: logits must be bfloat16, float16 or float32");
@@ -213,8 +218,7 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::
   if (vocab < 1 || vocab > cols) bad("token_logprobs: vocab must be between 1 and the logits' " + std::to_string(cols) + " columns");
   if (cols > wb::kLogprobMaxColumns || tokens.numel() >= std::numeric_limits<int32_t>::max())
     bad("token_logprobs: at most 2^30 columns and 2^31 - 2 rows");
-  if (!(temperature > 0) || !std::isfinite(temperature) || !std::isfinite((float)(1.0 / temperature)) || (float)(1.0 / temperature) == 0.f)
-    bad("token_logprobs: the temperature must be positive and finite");
+  if (!(temperature >= 1e-30 && temperature <= 1e30)) bad("token_logprobs: the temperature must be between 1e-30 and 1e30");
   if (top_k < 0 || top_k > wb::kLogprobMaxTop || top_k > vocab)
     bad("token_logprobs: top_k must be between 0 and " + std::to_string(std::min<int64_t>(wb::kLogprobMaxTop, vocab)));
   if (top_k && vocab > wb::kLogprobMaxTopVocab)
@@ -258,6 +262,7 @@ py::tuple sum_squares(const py::object& tensors) {
     if (!THPVariable_Check(o)) throw py::type_error("grad_norm: not a tensor");
     const Tensor& x = THPVariable_Unpack(o);
     if (!first) first = &x;
+    if (wrapped(x)) bad(std::string("grad_norm: a tensor") + kWrapped);
     if (!x.is_cuda() || x.device() != first->device()) bad("grad_norm: all tensors must be CUDA tensors of one device");
     if (!float_code(x.scalar_type())) bad("grad_norm: tensors must be bfloat16, float16 or float32");
     if (!dense(x)) bad("grad_norm: a tensor of shape " + shape_of(x) + " has holes or overlaps in memory");
@@ -359,6 +364,7 @@ struct AdamWProgram {
   }
 
   void check_param(const Tensor& p, const std::string& name) const {
+    if (wrapped(p)) bad("AdamW: " + name + kWrapped);
     if (!p.is_cuda() || p.device() != dev) bad("AdamW: " + name + " is not on the CUDA device of the first parameter");
     if (!float_code(p.scalar_type())) bad("AdamW: " + name + " must be bfloat16, float16 or float32");
     if (!dense(p)) bad("AdamW: " + name + " has holes or overlaps in memory; give the whole parameter, not a view of part of it");
@@ -466,6 +472,7 @@ struct AdamWProgram {
         g = &p.grad();
       }
       if (!g || !g->defined()) continue;
+      if (wrapped(*g)) bad("AdamW.step: the gradient of " + names[i] + kWrapped);
       if (!g->is_cuda() || g->device() != dev) bad("AdamW.step: the gradient of " + names[i] + " is on another device");
       if (g->sizes() != p.sizes()) bad("AdamW.step: the gradient of " + names[i] + " has shape " + shape_of(*g) + ", not " + shape_of(p));
       if (g->scalar_type() != p.scalar_type() && g->scalar_type() != at::kFloat)

@@ -16,7 +16,8 @@ def grad_norm(tensors: Mapping[str, torch.Tensor] | Iterable[torch.Tensor], grou
     """The 2-norm over all ``tensors`` (a dict or an iterable; ``None`` entries are left out) as
     an fp32 scalar on their device, without waiting for it.
 
-    bf16, fp16 and fp32 tensors of one device, each filling its memory without holes.  The sum
+    bf16, fp16 and fp32 tensors of one device, each filling its memory without holes (of a DTensor,
+    its local tensor).  The sum
     runs in a fixed order: the same inputs give the same bits.  ``group``: a process group over
     which the squares are summed; a tensor that several of its ranks hold counts once per rank.
     Squares are formed in 32 bits: a gradient above 1.8e19 makes the norm infinite.
@@ -36,7 +37,8 @@ class AdamW:
 
     ``params``: name -> tensor, e.g. ``dict(model.named_parameters())`` or the tensors a layout
     allocates; bf16, fp16 or fp32 on one CUDA device, each filling its memory without holes (any
-    order of dimensions).  They are updated in place.  ``states``: ``"fp32"``, or ``"fp8"``:
+    order of dimensions).  They are updated in place.  Of an FSDP trainer's DTensors, their local
+    tensors (``parallel.fsdp.convert_to_wb`` returns those) with the gradients' local tensors.  ``states``: ``"fp32"``, or ``"fp8"``:
     both moments as e4m3 with one fp32 scale per 128 elements, 2.06 bytes a parameter instead of
     8 (the second moment as its root).  An 8-bit second moment follows changes of a few percent a
     step only through its block's largest element: use a ``beta2`` of at most 0.99 with it.
@@ -46,7 +48,8 @@ class AdamW:
 
     The states are flat buffers (``states()``); every tensor's slice starts at a multiple of 128
     elements, in the order of ``params``.  The step count lives on the device, so a captured step
-    can be replayed.
+    can be replayed; a step runs on the current stream of the parameters' device.  fp32 arithmetic
+    with the hardware's approximate root and reciprocal (relative errors of 2^-23).
     """
 
     def __init__(self, params: Mapping[str, torch.Tensor], lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
@@ -56,8 +59,8 @@ class AdamW:
             raise ValueError(f"AdamW: states must be 'fp32' or 'fp8', not {states!r}")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"AdamW: betas must be in [0, 1), not {betas}")
-        if not eps > 0.0 or not weight_decay >= 0.0:
-            raise ValueError("AdamW: eps must be positive and weight_decay not negative")
+        if not 2.0 ** -126 <= eps < float("inf") or not 0.0 <= weight_decay < float("inf"):
+            raise ValueError("AdamW: eps must be a positive normal fp32 number and weight_decay not negative")
         self._check_lr(lr)
         self.lr = lr
         self.betas, self.eps, self.weight_decay = tuple(map(float, betas)), float(eps), float(weight_decay)
@@ -71,8 +74,8 @@ class AdamW:
 
     @staticmethod
     def _check_lr(lr) -> None:
-        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
-            raise ValueError(f"AdamW: lr must not be negative, not {lr}")
+        if not isinstance(lr, torch.Tensor) and not 0.0 <= lr < float("inf"):
+            raise ValueError(f"AdamW: lr must be finite and not negative, not {lr}")
 
     def step(self, grads: Mapping[str, torch.Tensor] | None = None, *, lr: float | torch.Tensor | None = None,
              max_norm: float | None = None, group: Any = None) -> torch.Tensor | None:
