@@ -209,9 +209,10 @@ struct States {
   }
 };
 
-// Elements a lane takes at once with vectors: eight, and sixteen of 8-bit states beside 16-bit
-// parameters and gradients (W: bytes of the parameter or master weight and the gradient).
-template <bool FP8, int W> constexpr int kLaneElems = FP8 && W <= 4 ? 16 : 8;
+// Elements a lane takes at once with vectors: eight, and sixteen of 8-bit states (one 16-byte load of
+// codes, eight lanes a block) unless parameter or master weight and gradient are both fp32 (W: their
+// bytes), which the copies' slots do not hold.
+template <bool FP8, int W> constexpr int kLaneElems = FP8 && W <= 6 ? 16 : 8;
 
 // One lane's vectors of a step; V: what the new value is computed from, the parameter's type or fp32.
 template <bool FP8, typename P, typename G, typename V>
@@ -236,7 +237,8 @@ struct Lane {
     #pragma unroll
     for (int i = 0; i < E / 2; ++i) update2(s, keep, grad[i], states.m[i], states.v[i], value[i], r[i]);
     if constexpr (!std::is_same_v<P, V>) store_pairs<E>(from, value);
-    store_pairs<E>(param, value);
+    if constexpr (FP8) store_pairs16<E>(param, value);
+    else store_pairs<E>(param, value);
     states.store(a, si, r);
   }
 };
@@ -245,7 +247,7 @@ struct Lane {
 // The arithmetic of sixteen elements needs the registers that a register prefetch would take.
 // Lanes copy 16 bytes side by side (every sector once) and read back their own elements, so a
 // warp's barrier stands after the wait for the copies and before a stage is filled again.
-constexpr int kStages = 3, kMaxSlots = 6;
+constexpr int kStages = 3, kMaxSlots = 8;
 constexpr size_t kStageBytes = (size_t)kStages * kMaxSlots * kThreads * 16;
 
 __device__ __forceinline__ void copy_async16(uint32_t to, const void* from) {
@@ -360,7 +362,8 @@ __device__ __forceinline__ void step_chunk(const AdamArgs& a, const StepScalars&
   const uint32_t lane = threadIdx.x & 31, off = lane * L::E;
   P* param = reinterpret_cast<P*>(t.param);
   const G* gp = reinterpret_cast<const G*>(grad);
-  const bool aligned = ((t.param | grad) & 31) == 0;
+  // 8-bit states: copies and stores of 16 bytes; otherwise vectors of 32
+  const bool aligned = ((t.param | grad) & (FP8 ? 15 : 31)) == 0;
   const uint32_t span = aligned ? kSpan : kOddSpan<FP8>;
   uint64_t i = begin + (threadIdx.x >> 5) * span;
   if (!aligned) {

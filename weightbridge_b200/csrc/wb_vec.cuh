@@ -181,6 +181,19 @@ __device__ __forceinline__ void store_pairs(T* p, const F2 (&x)[E / 2]) {
   }
 }
 
+// The same for addresses aligned to 16 bytes only.
+template <int E, typename T>
+__device__ __forceinline__ void store_pairs16(T* p, const F2 (&x)[E / 2]) {
+  constexpr int N = 16 / (int)sizeof(T);
+  #pragma unroll
+  for (int k = 0; k < E / N; ++k) {
+    F2 part[N / 2];
+    #pragma unroll
+    for (int i = 0; i < N / 2; ++i) part[i] = x[k * (N / 2) + i];
+    store_pairs<N>(p + k * N, part);
+  }
+}
+
 // 2^x by the hardware's approximation (relative error 2^-22; results below 2^-126 become 0).
 __device__ __forceinline__ float ex2(float x) {
   float r;
