@@ -542,7 +542,9 @@ __device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base
   __syncthreads();
 }
 
-// A CTA per row, or a cluster of `splits` CTAs.
+// A CTA per row, or a cluster of `splits` CTAs.  4096 x 128256 bf16: 177 to 187 us, 0.92 to 0.87 of the
+// measured copy rate (one of two GPUs, the other); 64 x 151936 with 20 alternatives: 15 us; one row of
+// 128256: 4.7 us, with 5 alternatives 7.7.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const LogprobRows in, const LogprobOut out, const uint32_t splits) {
   extern __shared__ __align__(16) uint32_t tops[];       // TOP: the tiles' maxima, and zeros up to a multiple of four
@@ -616,7 +618,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const Logprob
 // -- gradient -------------------------------------------------------------------------------------
 constexpr uint32_t kGradTiles = 16;        // tiles of one warp's work: 16 KiB read, 16 KiB written
 
-// Reads a logit and writes a gradient, once each, at HBM's rate; a warp takes up to 16 tiles of one
+// Reads a logit and writes a gradient, once each, at HBM's rate (4096 x 152064 bf16: 400 us, 0.96 of
+// the measured copy rate); a warp takes up to 16 tiles of one
 // row and shares nothing.  Tiles follow the gradient's alignment.  Where the logits' rows lie
 // otherwise (views whose rows are not multiples of 32 bytes), and at the ends of a row, lanes take
 // single elements side by side instead of vectors.

@@ -11,6 +11,9 @@
 // block has to span (e4m3 holds 2^-9 .. 448, so v spans 2^35 within a block).  A positive r never
 // takes the code 0 but at least the smallest, 2^-9: a zero denominator would let the step grow
 // without bound, a denominator rounded up only shortens it.
+// What bounds it: HBM.  Of the measured copy rate, over 200M elements: fp32 states 0.94 to 0.98 (0.85 to
+// 0.95 at odd addresses), 8-bit states 0.83 to 0.89 (0.46 to 0.76): their arithmetic, 29 instructions
+// an element, runs close behind.  The norm: 604M bf16 gradients in 174 us, as fast as they are read.
 #include "wb_optim.h"
 
 #include <cuda_fp8.h>
