@@ -113,7 +113,7 @@ def _step_and_check(params, grads, opt, lr=1e-2, max_norm=None, wd=0.1, no_decay
 
 @gpu
 @pytest.mark.parametrize("states", ["fp32", "fp8"])
-@pytest.mark.parametrize("shift", [0, 1, 3])
+@pytest.mark.parametrize("shift", [0, 1, 3, 4, 8])
 @pytest.mark.parametrize("dtype,gdtype,master", [
     (torch.float32, None, False), (torch.bfloat16, None, False), (torch.bfloat16, torch.float32, True), (torch.bfloat16, torch.float32, False),
     (torch.float16, None, True), (torch.float16, torch.float32, False)])
@@ -210,6 +210,22 @@ def test_extreme_gradients_in_8_bit_blocks():
     assert bool((st["exp_avg_scale"] > 0).all()) and bool((st["rms"].float()[256:384] > 0).all())
     assert bool((params["p"] < 1).all())                        # even the zeros decayed, and nothing blew up
     assert float((params["p"] - 1).abs().max()) < 0.5
+
+
+@gpu
+def test_infinite_gradients_without_clipping_stay_visible():
+    """No norm, no check: the parameter turns NaN as in 32 bits, and the block's moments do not turn into numbers again."""
+    for states in ("fp32", "fp8"):
+        params = {"p": torch.ones(256, device="cuda")}
+        opt = AdamW(params, states=states)
+        g = torch.ones(256, device="cuda")
+        g[3] = math.inf
+        opt.step({"p": g})
+        g[3] = 1.0
+        opt.step({"p": g})
+        p = params["p"]
+        assert not math.isfinite(float(p[3])) and bool(p[128:].isfinite().all())
+        assert not bool(opt.states()["exp_avg_scale" if states == "fp8" else "exp_avg"][:128].isfinite().all())
 
 
 @gpu

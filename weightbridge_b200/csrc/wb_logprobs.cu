@@ -12,7 +12,8 @@
 // Forward: one pass.  A warp takes tiles of 1 KiB (32 bytes a lane), two loads under way; every lane
 // keeps its own sums.  What bounds it is HBM, with the exponentials (16 a clock and SM: 16-bit
 // logits arrive at 0.7 of their rate) and the instructions around them close behind, so the common
-// path takes five an element: no running maximum, no clamp.  A row that needs them is read again.
+// path takes no running maximum and no clamp (194 -> 186 us for 4096 x 128256 bf16).  A row that needs
+// them is read again.
 // A CTA of eight warps takes a row; where rows are few, a cluster of CTAs shares one and joins
 // through distributed shared memory (no workspace, no second launch).
 //

@@ -27,18 +27,6 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr double kMaxDouble = 1.7976931348623157e308;
 
-__device__ __forceinline__ float load_as_f32(uint64_t p, uint32_t dtype, uint64_t i) {
-  if (dtype == DT_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
-
-__device__ __forceinline__ void store_from_f32(uint64_t p, uint32_t dtype, uint64_t i, float x) {
-  if (dtype == DT_F32) reinterpret_cast<float*>(p)[i] = x;
-  else if (dtype == DT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
-  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
-}
-
 // A sum over the CTA in a fixed order; all threads get it.
 __device__ __forceinline__ double cta_sum(double v, double* red) {
   v = warp_sum(v);
@@ -99,6 +87,7 @@ __device__ __forceinline__ float block_scale(float amax) {
   constexpr float kInv = 1.f / kE4M3Max;
   float q = amax * kInv;
   q = fmaf(fmaf(-kE4M3Max, q, amax), kInv, q);
+  if (!(amax <= 3.402823466e38f)) q = amax;              // an infinite moment stays one
   return amax > 0.f ? fmaxf(q, 1.17549435e-38f) : 1.f;
 }
 __device__ __forceinline__ float block_inverse(float amax) {
@@ -114,30 +103,19 @@ __device__ __forceinline__ F2 root_codes(F2 r, float inv) {
   return {fmaxf(q.x, r.x > 0.f ? 0.001953125f : 0.f), fmaxf(q.y, r.y > 0.f ? 0.001953125f : 0.f)};
 }
 
-// What one lane loads of the states of E consecutive elements, as it comes from memory.
+// The states of E consecutive elements of one lane as they come from memory.
 template <bool FP8, int E> struct RawStates;
 
 template <int E>
 struct RawStates<true, E> {
-  uint32_t m[E / 4], v[E / 4];
+  uint32_t m[E / 4], v[E / 4];              // codes
   float ms, vs;
   __device__ __forceinline__ void load(const AdamArgs& a, uint64_t si) {
-    read(reinterpret_cast<const uint8_t*>(a.m) + si, m);
-    read(reinterpret_cast<const uint8_t*>(a.v) + si, v);
+    static_assert(E == 4);                  // longer ones come through shared memory
+    m[0] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(a.m) + si);
+    v[0] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(a.v) + si);
     ms = a.m_scale[si / kStateBlock];
     vs = a.v_scale[si / kStateBlock];
-  }
-  __device__ __forceinline__ static void read(const uint8_t* p, uint32_t (&q)[E / 4]) {
-    if constexpr (E == 16) {
-      const uint4 w = load16(p);
-      q[0] = w.x, q[1] = w.y, q[2] = w.z, q[3] = w.w;
-    } else if constexpr (E == 8) {
-      const uint2 w = load8(p);
-      q[0] = w.x, q[1] = w.y;
-    } else {
-      static_assert(E == 4);
-      q[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
   }
 };
 
@@ -365,8 +343,8 @@ __device__ __forceinline__ void step_chunk(const AdamArgs& a, const StepScalars&
   const uint32_t lane = threadIdx.x & 31, off = lane * L::E;
   P* param = reinterpret_cast<P*>(t.param);
   const G* gp = reinterpret_cast<const G*>(grad);
-  // 8-bit states: copies and stores of 16 bytes; otherwise vectors of 32
-  const bool aligned = ((t.param | grad) & (FP8 ? 15 : 31)) == 0;
+  // 8-bit states: copies and stores of 16 bytes; otherwise vectors of eight elements
+  const bool aligned = (t.param & (FP8 ? 15 : 8 * sizeof(P) - 1)) == 0 && (grad & (FP8 ? 15 : 8 * sizeof(G) - 1)) == 0;
   const uint32_t span = aligned ? kSpan : kOddSpan<FP8>;
   uint64_t i = begin + (threadIdx.x >> 5) * span;
   if (!aligned) {
