@@ -268,6 +268,12 @@ def test_partial_gradients_none_and_second_derivative():
     only_lp, = torch.autograd.grad(out.logprobs.sum(), leaf, retain_graph=True)
     both, = torch.autograd.grad(out.entropy.sum() + out.logprobs.sum(), leaf, retain_graph=True)
     assert torch.allclose(only_h + only_lp, both, rtol=1e-5, atol=1e-6)
+    changed = x.clone().requires_grad_()
+    view = changed * 1.0
+    late = token_logprobs(view, t).logprobs.sum()
+    view.detach().zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        late.backward()
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(out.logprobs.sum(), leaf, create_graph=True)
     shared = torch.randn(1, 300, device="cuda", requires_grad=True)          # broadcast input: gradients add up

@@ -163,6 +163,17 @@ def test_parameters_own_gradients_and_versions():
 
 
 @gpu
+def test_inference_tensors_and_no_elements():
+    with torch.inference_mode():
+        p = {"p": torch.ones(300, device="cuda")}
+        AdamW(p, lr=0.5, weight_decay=0.0).step({"p": torch.ones(300, device="cuda")})
+        assert float((p["p"] - 0.5).abs().max()) < 1e-6
+    for states in ("fp32", "fp8"):
+        opt = AdamW({"e": torch.empty(0, 5, device="cuda")}, states=states)
+        assert float(opt.step({"e": torch.empty(0, 5, device="cuda")}, max_norm=1.0)) == 0.0 and opt.step_count == 1
+
+
+@gpu
 @pytest.mark.parametrize("states", ["fp32", "fp8"])
 def test_transposed_parameters(states):
     base = _rand((130, 257), torch.float32, 3)
@@ -358,6 +369,8 @@ def test_refusals_on_the_gpu():
         opt.step({"a": g.to_sparse()})
     with pytest.raises(ValueError, match="sparse"):
         grad_norm([g.to_sparse()])
+    with pytest.raises(ValueError, match="max_norm, too"):
+        opt.step({"a": g}, group=object())
     with pytest.raises(ValueError, match="one value per element"):
         opt.slices(torch.zeros(3))
     for tensors, match in (([], "no tensors"), ([g.long()], "bfloat16"), ([g, g.cpu()], "device"), ([g[:, :3]], "holes")):

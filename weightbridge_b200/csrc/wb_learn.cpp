@@ -548,7 +548,8 @@ struct AdamWProgram {
     a.eps = eps;
     a.max_norm = max_norm;
     check(wb::launch_adamw(a, grads.data(), chunk_start.data(), sms, c10::cuda::getCurrentCUDAStream()), "AdamW launch");
-    for (const Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();
+    for (const Tensor& p : params)
+      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();       // autograd sees the change
     return norm.defined() ? py::cast(norm) : py::none();
   }
 

@@ -545,7 +545,7 @@ __device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base
 
 // A CTA per row, or a cluster of `splits` CTAs.  4096 x 128256 bf16: 177 to 187 us, 0.92 to 0.87 of the
 // measured copy rate (one of two GPUs, the other); 64 x 151936 with 20 alternatives: 15 us; one row of
-// 128256: 4.7 us, with 5 alternatives 7.7.
+// 128256: 4.8 us, with 5 alternatives 8.3.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const LogprobRows in, const LogprobOut out, const uint32_t splits) {
   extern __shared__ __align__(16) uint32_t tops[];       // TOP: the tiles' maxima, and zeros up to a multiple of four

@@ -95,6 +95,8 @@ class AdamW:
         on_device = lr if isinstance(lr, torch.Tensor) else None
         number = 0.0 if on_device is not None else float(lr)
         if max_norm is None:
+            if group is not None:
+                raise ValueError("AdamW.step: a group is for the norm: give max_norm, too")
             return p.step(grads, number, on_device, None, 0.0)
         if not max_norm > 0.0:
             raise ValueError(f"AdamW.step: max_norm must be positive, not {max_norm}")
