@@ -432,14 +432,14 @@ __device__ Selection select_first(uint32_t k, uint32_t low, uint32_t high, uint3
   return {low, from};
 }
 
-// Ranks n distinct candidates by counting; the first k go to `out` in order.
+// Ranks n distinct candidates (and zeros, which are none) by counting; the first k go to `out` in order.
 __device__ __forceinline__ void rank_candidates(const uint64_t* c, uint32_t n, uint32_t k, uint64_t* out) {
   for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = c[i];
     uint32_t rank = 0;
-    #pragma unroll 4
+    #pragma unroll 8
     for (uint32_t j = 0; j < n; ++j) rank += c[j] > mine;
-    if (rank < k) out[rank] = mine;
+    if (mine && rank < k) out[rank] = mine;
   }
 }
 
@@ -544,8 +544,8 @@ __device__ void find_top(const T* x, uint32_t vocab, uint32_t mis, uint32_t base
 }
 
 // A CTA per row, or a cluster of `splits` CTAs.  4096 x 128256 bf16: 177 to 187 us, 0.92 to 0.87 of the
-// measured copy rate (one of two GPUs, the other); 64 x 151936 with 20 alternatives: 15 us; one row of
-// 128256: 4.8 us, with 5 alternatives 8.3.
+// measured copy rate (one of two GPUs, the other); 64 x 151936 with 20 alternatives: 14.5 us; one row of
+// 128256: 4.7 us, with 5 alternatives 7.6.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const LogprobRows in, const LogprobOut out, const uint32_t splits) {
   extern __shared__ __align__(16) uint32_t tops[];       // TOP: the tiles' maxima, and zeros up to a multiple of four
@@ -586,18 +586,18 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const Logprob
     cl.sync();
     if (split == 0) {
       all = warp_join(lane < splits ? *cl.map_shared_rank(&mine, lane) : RowStats{kLowest, 0.f, 0.f}, c2);
-      if constexpr (TOP) {               // at most 8 * 32 candidates, a thread each
+      if constexpr (TOP) {               // at most 8 * 32 candidates, a thread each; 0: none
         const uint32_t k = (uint32_t)out.top_k, s = threadIdx.x / k, i = threadIdx.x % k;
         uint64_t c = 0;
         if (s < splits) {
           const TopShared* theirs = cl.map_shared_rank(&shared, s);
-          if (i < theirs->n_out) c = theirs->out[i];
+          const uint32_t n = theirs->n_out;
+          c = theirs->out[i];
+          if (i >= n) c = 0;
+          shared.candidates[threadIdx.x] = c;
         }
-        if (threadIdx.x == 0) shared.n_candidates = 0;
         __syncthreads();                 // this CTA's own list has been read, too
-        if (c) shared.candidates[atomicAdd(&shared.n_candidates, 1u)] = c;
-        __syncthreads();
-        rank_candidates(shared.candidates, shared.n_candidates, k, shared.out);
+        rank_candidates(shared.candidates, splits * k, k, shared.out);
         __syncthreads();
       }
     }
