@@ -254,6 +254,23 @@ def test_second_moment_keeps_up_in_8_bits():
 
 
 @gpu
+@pytest.mark.parametrize("shift", [0, 1])
+def test_elements_beyond_32_bit_offsets(shift):
+    """2^31 + 333 parameters in one tensor: the first step is lr along the gradient's sign, at both ends."""
+    n = 2 ** 31 + 333
+    flat, grad = (torch.zeros(n + shift, dtype=torch.bfloat16, device="cuda")[shift:] for _ in range(2))
+    grad[:1000] = 2.0 ** -10
+    grad[-1000:] = -2.0 ** -10
+    opt = AdamW({"p": flat}, lr=0.25, weight_decay=0.0, states="fp8")
+    norm = opt.step({"p": grad}, max_norm=1e9)
+    assert abs(float(norm) - 2.0 ** -10 * math.sqrt(2000)) < 1e-6
+    assert abs(float(grad_norm([grad])) - float(norm)) < 1e-9
+    for part, want in ((flat[:1000], -0.25), (flat[-1000:], 0.25), (flat[1000:2000], 0.0), (flat[2 ** 31 - 5000:2 ** 31 - 4000], 0.0)):
+        assert float((part.float() - want).abs().max()) < 1e-3       # half a step of bf16 at 0.25 is 2^-11
+    assert int((flat != 0).sum()) == 2000
+
+
+@gpu
 def test_thousands_of_tensors_take_several_launches():
     n = 4100
     params = {f"p{i}": _rand((1 + i % 13,), torch.float32, i) for i in range(n)}
