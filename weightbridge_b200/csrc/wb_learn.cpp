@@ -322,10 +322,12 @@ struct AdamWProgram {
     }
     const c10::cuda::CUDAGuard guard(dev);
     sms = sm_count(dev.index());
-    // A work item: up to eight tiles, as long as every SM gets sixteen items.  A CTA reads a tensor's
-    // entry once per item and overlaps its loads within it; small models need the CTAs instead.
-    chunk = 8 * wb::kAdamTile;
-    while (chunk > wb::kAdamTile && total < (int64_t)sms * 16 * chunk) chunk /= 2;
+    // A work item: one tile with fp32 states (436M parameters: 2099 us with one, 2120 with eight; 1.45M: 7.7
+    // and 12.4).  8-bit states overlap their loads within an item: eight tiles, as long as every SM
+    // gets 32 items (604M parameters: 1340 us with one, 1085 with eight, 1101 with sixteen; 24M:
+    // 105 with one, 117 with eight).
+    chunk = fp8 ? 8 * wb::kAdamTile : wb::kAdamTile;
+    while (chunk > wb::kAdamTile && total < (int64_t)sms * 32 * chunk) chunk /= 2;
     for (const Tensor& p : params) {
       chunk_start.push_back((uint32_t)n_chunks);
       n_chunks += ((uint64_t)p.numel() + chunk - 1) / chunk;
