@@ -315,6 +315,18 @@ def test_rows_that_outgrow_their_beginning(dtype, vocab):
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [616, 20000])
+def test_jumps_of_every_size(vocab):
+    """A late column J nats above the others, J = 1 .. 96: neither sum loses bits to the reference's distance."""
+    x, t = _inputs(96, vocab, torch.float32, seed=13, std=1.0)
+    x[:, -40] = x[:, :-40].amax(1) + torch.arange(1, 97, device="cuda")
+    x[:, -7] = x[:, -40] - 1.5
+    t[::2] = vocab - 40
+    _check(x, t, top_k=3)
+    _check(x * 0.31, t, temperature=0.31, grad=False)
+
+
+@gpu
 def test_no_rows():
     x = torch.randn(0, 64, device="cuda", requires_grad=True)
     out = token_logprobs(x, torch.zeros(0, dtype=torch.long, device="cuda"), top_k=3)
