@@ -1,0 +1,35 @@
+"""AdamW and the gradient norm at the limits of their arithmetic, of their kernels and of what a call may be given.
+
+Tolerances are those of ``test_optim.py``, which derives them.
+"""
+import math
+
+import pytest
+import torch
+
+from weightbridge_b200 import AdamW, grad_norm
+
+from .test_optim import _rand, _setup, _step_and_check, gpu
+
+
+@gpu
+@pytest.mark.parametrize("states", ["fp32", "fp8"])
+@pytest.mark.parametrize("shift", [0, 3])
+def test_the_same_bits_every_time(states, shift):
+    """Three steps, with another optimizer's steps between them and without: parameters, states and norms agree bit for bit."""
+    sizes = [(1500001,), (300, 517), (70001,), (128,), (5,)]
+
+    def make(seed=21):
+        return _setup(sizes, torch.float32, shift=shift, seed=seed, states=states)
+
+    a, ga, x = make()
+    b, gb, y = make()
+    c, gc, other = make(seed=40)
+    for k in range(3):
+        norms = x.step(ga, max_norm=None if k == 1 else 0.5), y.step(gb, max_norm=None if k == 1 else 0.5)
+        other.step(gc)
+        assert norms[0] is None and norms[1] is None or torch.equal(*norms)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, b[n]) for n, p in a.items())
+    for p, q in zip(x.states().values(), y.states().values()):
+        assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
