@@ -288,8 +288,9 @@ struct Walk {
 
   // Ordinary rows: the first tile's largest gives the reference of the whole walk, which is lifted
   // where a sum outgrows it, so no maximum is taken of the other tiles.  False (for the whole warp) at
-  // the first sum that is not finite (a masked column: 0 * -inf; NaN), or where a logit is some 2^35
-  // times as probable as the reference: A, of terms e^z z, would lose the bits of z to it.
+  // the first sum that is not finite (a masked column: 0 * -inf; NaN), where a logit is some 2^35
+  // times as probable as the reference (A, of terms e^z z, would lose the bits of z to it), or where the
+  // reference was lifted out of its range.
   template <bool TOP>
   __device__ __forceinline__ bool common(Stats& st, float c2, uint32_t base, uint32_t* tops) {
     if (first >= end) return true;
@@ -317,7 +318,9 @@ struct Walk {
       if (__any_sync(kFullWarp, !(fabsf(size) < 1.0995116e12f))) return false;       // 2^40
       if (size > 65536.f) lift(st);
     }
-    st.m = st.ref.b / c2;                  // reference(m) gives b again: |b| < 2^21
+    // reference(b / c2) gives b again: within 2^20 the quotient and its product are off by less than 1/8
+    if (__any_sync(kFullWarp, !(fabsf(st.ref.b) < kModerate))) return false;
+    st.m = st.ref.b / c2;
     return true;
   }
 
