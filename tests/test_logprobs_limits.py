@@ -27,3 +27,18 @@ def test_references_near_their_limit(rows, vocab, temperature):
             t = torch.full((rows,), vocab - 1, device="cuda")
             t[1::2] = 5
             _check(x, t, temperature=temperature)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1000, 20000, 60001])
+def test_no_log_probability_above_0_and_no_entropy_below(dtype, vocab):
+    """One column holds nearly all of the probability: both results are 0 but for their rounding, whose sign is known."""
+    x, t = _inputs(400, vocab, dtype, seed=14, std=1.0)
+    x[:, -3] = torch.linspace(12, 40, 400, device="cuda").to(dtype)
+    t[:] = vocab - 3
+    for part in (slice(0, 400), slice(0, 7)):
+        out = _check(x[part], t[part], top_k=2, grad=part.stop == 7)
+        assert not bool((out.logprobs > 0).any()) and not bool((out.top_logprobs > 0).any()) and not bool((out.entropy < 0).any())
+    out = _check(x, t)
+    assert not bool((out.logprobs > 0).any()) and not bool((out.entropy < 0).any())

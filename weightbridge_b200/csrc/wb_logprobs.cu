@@ -2,12 +2,16 @@
 // probable alternatives, and the gradient of the first two (sm_100a).
 //
 // Row x with V valid columns, temperature T:  m = max x,  z_j = (x_j - m) / T <= 0,
-//   S = sum e^z_j,  A = sum e^z_j z_j,  logp_j = z_j - ln S,  H = ln S - A / S  (both sums have one
-// sign, so nothing cancels), and with incoming gradients g (log probability) and h (entropy)
+//   S = sum e^z_j,  A = sum e^z_j z_j,  logp_j = z_j - ln S,  H = ln S - A / S,
+// and with incoming gradients g (log probability) and h (entropy)
 //   dx_j = ((j == token) g - p_j (g + h (logp_j + H))) / T.
 // A column of -inf has probability 0 and adds nothing to H.  A row without any finite column is
 // empty: log probability -inf, entropy 0, no gradient.  NaN and +inf make the row's results NaN.
 // Rows of the type's lowest value neither overflow nor become empty.  Every sum is held in 32 bits.
+// Counted from the maximum both sums have one sign and nothing cancels.  The common path counts from
+// the first tile's: where one column far above that holds nearly all of the probability, ln S and A / S
+// are alike and large, and their difference is off by up to 35 ln 2 half steps a term (some 1e-6).  The
+// signs are known, so no log probability comes out above 0 and no entropy below.
 //
 // Forward: one pass.  A warp takes tiles of 1 KiB (32 bytes a lane), two loads under way; every lane
 // keeps its own sums.  What bounds it is HBM, with the exponentials (16 a clock and SM: 16-bit
@@ -198,6 +202,7 @@ __device__ __forceinline__ RowResult finish(RowStats t, float c2) {
   r.ref = reference(r.m, c2);
   r.log2_sum = empty ? kInf : log2f(t.s);
   r.entropy = empty ? 0.f : kLn2 * (r.log2_sum - t.a / t.s);
+  if (r.entropy < 0.f) r.entropy = 0.f;    // rounding alone; NaN stays
   return r;
 }
 
@@ -205,7 +210,8 @@ __device__ __forceinline__ RowResult finish(RowStats t, float c2) {
 // is nothing beside it.
 __device__ __forceinline__ float logprob(const RowResult& t, float x, float c2) {
   const float z = t.ref.z(x, c2);
-  return z == -kInf && t.log2_sum < kInf ? (x - t.m) * (c2 * kLn2) : kLn2 * (z - t.log2_sum);
+  const float lp = z == -kInf && t.log2_sum < kInf ? (x - t.m) * (c2 * kLn2) : kLn2 * (z - t.log2_sum);
+  return lp > 0.f ? 0.f : lp;              // rounding alone; NaN stays
 }
 
 // The token's logit, loaded before the row: its latency passes under the row's.
