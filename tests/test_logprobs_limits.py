@@ -42,3 +42,27 @@ def test_no_log_probability_above_0_and_no_entropy_below(dtype, vocab):
         assert not bool((out.logprobs > 0).any()) and not bool((out.top_logprobs > 0).any()) and not bool((out.entropy < 0).any())
     out = _check(x, t)
     assert not bool((out.logprobs > 0).any()) and not bool((out.entropy < 0).any())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [500, 501])
+@pytest.mark.parametrize("temperature,scale", [(1e-4, 2.0 ** 17), (1e-6, 2.0 ** 16), (1e-9, 1.0), (1e-12, 1.0), (1e-20, 1.0), (1e-30, 1.0), (1e-30, 1e6)])
+def test_gradient_at_small_temperatures(dtype, vocab, temperature, scale):
+    """Columns without any probability get no gradient, however large 1 / temperature and the incoming gradients are."""
+    x, t = _inputs(6, vocab, dtype, seed=15)
+    x[0, ::2] = -math.inf
+    x[1, 3:] = torch.finfo(dtype).min
+    x[2, 5] = x[2, 7] = 30.0                                     # two largest
+    x[3] = 0.0
+    x[3, 4] = -math.inf
+    t[2], t[4] = 7, int(x[4].argmax())
+    x = x[:, :vocab].detach().requires_grad_()
+    out = token_logprobs(x, t, temperature=temperature)
+    lp, h, logp, keep, z, p = _oracle(x, t, vocab, temperature)
+    tol_lp, tol_h = _bounds(z, p, lp, vocab)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    g1, g2 = (torch.randn(6, device="cuda", generator=g) * scale for _ in range(2))
+    d, = torch.autograd.grad((out.logprobs, out.entropy), x, (g1, g2))
+    assert bool(d.isfinite().all())
+    _check_grad(d, g1, g2, lp, h, logp, p, keep, t, vocab, temperature, tol_lp, tol_h)

@@ -660,10 +660,15 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_grad_kernel(const Logpro
     const F2 z = fma2(v, F2{c2, c2}, F2{-b, -b});
     return mul2(F2{ex2(z.x), ex2(z.y)}, fma2(F2{d1, d1}, z, F2{c1, c1}));
   };
-  auto safe2 = [&](F2 v) {                               // as in accumulate()
+  // Any column: one without probability gets 0, whatever c and d z are (1 / T and the incoming gradients may
+  // be so large that these pass the range).  NaN stays.
+  auto safe2 = [&](F2 v) {
     const F2 z = fma2(add2(v, F2{-a, -a}), F2{c2, c2}, F2{-b, -b});
-    return mul2(F2{ex2(z.x), ex2(z.y)}, fma2(F2{d1, d1}, F2{fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)}, F2{c1, c1}));
+    const F2 p{ex2(z.x), ex2(z.y)}, d = mul2(p, fma2(F2{d1, d1}, z, F2{c1, c1}));
+    return F2{p.x == 0.f ? 0.f : d.x, p.y == 0.f ? 0.f : d.y};
   };
+  // of an ordinary reference and logits above `lowest` |z| is below 2^22
+  const bool plain = ref.ordinary() && fabsf(d1) < 1.2676506e30f && fabsf(c1) < 1.7014118e38f;   // 2^100, 2^127
   const bool vectors = misaligned(x) == mis;
   const uint32_t tiles = (mis + g.cols + kTile<T> - 1) / kTile<T>;
   const uint32_t begin = seg * kGradTiles, end = min(begin + kGradTiles, tiles);
@@ -678,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_grad_kernel(const Logpro
         for (int i = 0; i < N / 2; ++i) v[i] = {0.f, 0.f};
       } else {
         unpack<T>(load32(x + j0), v);
-        if (ref.ordinary() && least(v) > lowest) {
+        if (plain && least(v) > lowest) {
           #pragma unroll
           for (int i = 0; i < N / 2; ++i) v[i] = plain2(v[i]);
         } else {
