@@ -66,3 +66,18 @@ def test_gradient_at_small_temperatures(dtype, vocab, temperature, scale):
     d, = torch.autograd.grad((out.logprobs, out.entropy), x, (g1, g2))
     assert bool(d.isfinite().all())
     _check_grad(d, g1, g2, lp, h, logp, p, keep, t, vocab, temperature, tol_lp, tol_h)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """They would be lost: the results would come out as constants."""
+    import torch.autograd.forward_ad as forward_ad
+    x, t = torch.randn(4, 10), torch.zeros(4, dtype=torch.long)
+
+    def refused(match, logits, tokens=t):
+        with pytest.raises(ValueError, match=match):
+            token_logprobs(logits, tokens)
+
+    with forward_ad.dual_level():
+        refused("forward mode", forward_ad.make_dual(x, torch.ones_like(x)))
+        refused("forward mode", forward_ad.make_dual(x, torch.ones_like(x)).clone().requires_grad_())
+        refused("forward mode", forward_ad.make_dual(torch.randn(5, 10), torch.ones(5, 10))[1:])

@@ -33,3 +33,16 @@ def test_the_same_bits_every_time(states, shift):
     assert all(torch.equal(p, b[n]) for n, p in a.items())
     for p, q in zip(x.states().values(), y.states().values()):
         assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
+
+
+@gpu
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as forward_ad
+    p, g = torch.ones(64, device="cuda"), torch.ones(64, device="cuda")
+    opt = AdamW({"a": p})
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(g, torch.ones_like(g))
+        for call in (lambda: AdamW({"a": dual}), lambda: opt.step({"a": dual}), lambda: grad_norm([dual])):
+            with pytest.raises(ValueError, match="forward mode"):
+                call()
+    assert opt.step_count == 0 and bool((p == 1).all())

@@ -48,9 +48,14 @@ std::string shape_of(const Tensor& t) {
   return s + "]";
 }
 
-// Wrappers of other tensors (DTensor and the like) have no memory of their own.
-bool wrapped(const Tensor& t) { return t.layout() != at::kStrided || t.key_set().has(c10::DispatchKey::Python); }
-constexpr const char* kWrapped = " is a sparse tensor or a wrapper (DTensor): give the plain local tensor (to_local())";
+// Why a tensor's memory may not be read as its values, or null.  Wrappers of other tensors (DTensor and
+// the like) have no memory of their own; a forward mode derivative would be lost without a word.
+const char* unfit(const Tensor& t) {
+  if (t.layout() != at::kStrided || t.key_set().has(c10::DispatchKey::Python))
+    return " is a sparse tensor or a wrapper (DTensor): give the plain local tensor (to_local())";
+  if (t._fw_grad(0).defined()) return " carries a derivative of forward mode, which is not implemented: give the primal";
+  return nullptr;
+}
 
 int sm_count(int device) {
   static std::array<int, 64> known{};          // one attribute query per device; the value never changes
@@ -208,7 +213,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 
 py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::optional<int64_t>& columns, double temperature,
                          int64_t top_k, int64_t ignore_index) {
-  if (wrapped(logits) || wrapped(tokens)) bad(std::string("token_logprobs: an argument") + kWrapped);
+  for (const Tensor* x : {&logits, &tokens})
+    if (const char* why = unfit(*x)) bad(std::string("token_logprobs: an argument") + why);
   if (logits.dim() < 1) bad("token_logprobs: logits need a vocabulary dimension");
   const int64_t cols = logits.size(-1), vocab = columns.value_or(cols);
   if (!float_code(logits.scalar_type())) bad("token_logprobs: logits must be bfloat16, float16 or float32");
@@ -262,7 +268,7 @@ py::tuple sum_squares(const py::object& tensors) {
     if (!THPVariable_Check(o)) throw py::type_error("grad_norm: not a tensor");
     const Tensor& x = THPVariable_Unpack(o);
     if (!first) first = &x;
-    if (wrapped(x)) bad(std::string("grad_norm: a tensor") + kWrapped);
+    if (const char* why = unfit(x)) bad(std::string("grad_norm: a tensor") + why);
     if (!x.is_cuda() || x.device() != first->device()) bad("grad_norm: all tensors must be CUDA tensors of one device");
     if (!float_code(x.scalar_type())) bad("grad_norm: tensors must be bfloat16, float16 or float32");
     if (!dense(x)) bad("grad_norm: a tensor of shape " + shape_of(x) + " has holes or overlaps in memory");
@@ -366,7 +372,7 @@ struct AdamWProgram {
   }
 
   void check_param(const Tensor& p, const std::string& name) const {
-    if (wrapped(p)) bad("AdamW: " + name + kWrapped);
+    if (const char* why = unfit(p)) bad("AdamW: " + name + why);
     if (!p.is_cuda() || p.device() != dev) bad("AdamW: " + name + " is not on the CUDA device of the first parameter");
     if (!float_code(p.scalar_type())) bad("AdamW: " + name + " must be bfloat16, float16 or float32");
     if (!dense(p)) bad("AdamW: " + name + " has holes or overlaps in memory; give the whole parameter, not a view of part of it");
@@ -474,7 +480,7 @@ struct AdamWProgram {
         g = &p.grad();
       }
       if (!g || !g->defined()) continue;
-      if (wrapped(*g)) bad("AdamW.step: the gradient of " + names[i] + kWrapped);
+      if (const char* why = unfit(*g)) bad("AdamW.step: the gradient of " + names[i] + why);
       if (!g->is_cuda() || g->device() != dev) bad("AdamW.step: the gradient of " + names[i] + " is on another device");
       if (g->sizes() != p.sizes()) bad("AdamW.step: the gradient of " + names[i] + " has shape " + shape_of(*g) + ", not " + shape_of(p));
       if (g->scalar_type() != p.scalar_type() && g->scalar_type() != at::kFloat)

@@ -38,8 +38,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, vocab: int | N
     empty: log probability -inf, entropy 0, gradient 0.  NaN or +inf in a row, or a token
     outside the vocabulary, make its log probability NaN.
 
-    Differentiable once in ``logits`` through ``logprobs`` and ``entropy``; the gradient has the
-    logits' type.  Results are fp32 and held in 32 bits throughout.  Runs on the current stream
+    Differentiable once in ``logits`` through ``logprobs`` and ``entropy``, in reverse mode (a tensor
+    with a forward mode derivative is refused); the gradient has the logits' type.  Results are fp32 and held in 32 bits throughout.  Runs on the current stream
     of the logits' device and can be captured into a CUDA graph.
     """
     return TokenLogprobs(*ext().token_logprobs(logits, tokens, vocab, temperature, top_k, ignore_index))
