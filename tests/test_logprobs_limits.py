@@ -81,3 +81,25 @@ def test_forward_mode_derivatives_are_refused():
         refused("forward mode", forward_ad.make_dual(x, torch.ones_like(x)))
         refused("forward mode", forward_ad.make_dual(x, torch.ones_like(x)).clone().requires_grad_())
         refused("forward mode", forward_ad.make_dual(torch.randn(5, 10), torch.ones(5, 10))[1:])
+
+
+def test_lazily_negated_tensors_are_refused():
+    """Their memory holds other values than they do."""
+    x, t = torch.randn(4, 10), torch.zeros(4, dtype=torch.long)
+    for logits, tokens in ((torch._neg_view(x), t), (torch.complex(x, x).conj().imag, t), (x, torch._neg_view(t))):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            token_logprobs(logits, tokens)
+
+
+@gpu
+def test_lazily_negated_gradient():
+    x, t = _inputs(5, 300, torch.float32)
+    x.requires_grad_()
+    out = token_logprobs(x, t)
+    g = torch.randn(5, device="cuda")
+    lazy = torch.complex(g, g).conj().imag                       # -g, with g's values in memory
+    assert lazy.is_neg()
+    for o in (out.logprobs, out.entropy):
+        d, = torch.autograd.grad(o, x, lazy, retain_graph=True)
+        want, = torch.autograd.grad(o, x, -g, retain_graph=True)
+        assert torch.equal(d, want)

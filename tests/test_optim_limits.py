@@ -46,3 +46,13 @@ def test_forward_mode_derivatives_are_refused():
             with pytest.raises(ValueError, match="forward mode"):
                 call()
     assert opt.step_count == 0 and bool((p == 1).all())
+
+
+@gpu
+def test_lazily_negated_tensors_are_refused():
+    p, g = torch.ones(64, device="cuda"), torch.ones(64, device="cuda")
+    opt = AdamW({"a": p})
+    for call in (lambda x: AdamW({"a": x}), lambda x: opt.step({"a": x}), lambda x: grad_norm([x])):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call(torch._neg_view(g))
+    assert opt.step_count == 0 and bool((p == 1).all())

@@ -53,6 +53,7 @@ std::string shape_of(const Tensor& t) {
 const char* unfit(const Tensor& t) {
   if (t.layout() != at::kStrided || t.key_set().has(c10::DispatchKey::Python))
     return " is a sparse tensor or a wrapper (DTensor): give the plain local tensor (to_local())";
+  if (t.is_neg()) return " is negated lazily, its memory holds other values: give resolve_neg() of it";
   if (t._fw_grad(0).defined()) return " carries a derivative of forward mode, which is not implemented: give the primal";
   return nullptr;
 }
@@ -160,7 +161,7 @@ LogprobResult run_logprobs(const Tensor& logits, const Tensor& tokens, const Log
 // A gradient over the rows as one stride (autograd hands expanded ones).
 Tensor row_grad(const Tensor& g, const float*& ptr, int64_t& stride) {
   if (!g.defined()) return g;
-  Tensor t = g.scalar_type() == at::kFloat ? g : g.to(at::kFloat);
+  Tensor t = g.to(at::kFloat).resolve_neg();             // the engine may hand a lazily negated one; both leave an ordinary one alone
   auto l = lead_of(t, t.dim());
   if (!l || l->outer != 1) {
     t = t.contiguous();
