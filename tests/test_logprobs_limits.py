@@ -103,3 +103,15 @@ def test_lazily_negated_gradient():
         d, = torch.autograd.grad(o, x, lazy, retain_graph=True)
         want, = torch.autograd.grad(o, x, -g, retain_graph=True)
         assert torch.equal(d, want)
+
+
+def test_tensors_of_transforms_are_refused():
+    """What torch.func hands to a function has no memory of its own (an address of 0 for some)."""
+    x, t = torch.randn(4, 10), torch.zeros(4, dtype=torch.long)
+    with pytest.raises(ValueError, match="wrapper"):
+        token_logprobs(torch._efficientzerotensor((4, 10)), t)
+    for transform in (torch.func.functionalize, torch.func.grad, torch.vmap):
+        with pytest.raises(ValueError, match="wrapper"):
+            transform(lambda y: token_logprobs(y, t if y.dim() == 2 else t[0]).logprobs.sum())(x)
+        with pytest.raises(ValueError, match="wrapper"):
+            transform(lambda y: token_logprobs(x, y).logprobs.sum())(t.float() if transform is torch.func.grad else t)

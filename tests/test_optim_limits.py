@@ -56,3 +56,13 @@ def test_lazily_negated_tensors_are_refused():
         with pytest.raises(ValueError, match="resolve_neg"):
             call(torch._neg_view(g))
     assert opt.step_count == 0 and bool((p == 1).all())
+
+
+def test_tensors_of_transforms_are_refused():
+    x = torch.ones(4)
+    for transform in (torch.func.functionalize, torch.func.grad, torch.vmap):
+        for call in (lambda y: AdamW({"a": y}), lambda y: grad_norm([y])):
+            with pytest.raises(ValueError, match="wrapper"):
+                transform(call)(x[0] if transform is torch.func.grad else x)
+    with pytest.raises(ValueError, match="wrapper"):
+        grad_norm([torch._efficientzerotensor((4,))])

@@ -48,11 +48,15 @@ std::string shape_of(const Tensor& t) {
   return s + "]";
 }
 
-// Why a tensor's memory may not be read as its values, or null.  Wrappers of other tensors (DTensor and
-// the like) have no memory of their own; a forward mode derivative would be lost without a word.
+// Why a tensor's memory may not be read as its values, or null.  Wrappers of other tensors (DTensor, what
+// torch.func hands to a function) and lazy zeros have no memory of their own, some an address of 0; a
+// forward mode derivative would be lost without a word.
 const char* unfit(const Tensor& t) {
-  if (t.layout() != at::kStrided || t.key_set().has(c10::DispatchKey::Python))
-    return " is a sparse tensor or a wrapper (DTensor): give the plain local tensor (to_local())";
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet kWrappers({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
+                                           DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched, DispatchKey::ZeroTensor});
+  if (t.layout() != at::kStrided || t.key_set().has_any(kWrappers))
+    return " is a sparse tensor or a wrapper (DTensor, a transform's): give the plain local tensor (to_local())";
   if (t.is_neg()) return " is negated lazily, its memory holds other values: give resolve_neg() of it";
   if (t._fw_grad(0).defined()) return " carries a derivative of forward mode, which is not implemented: give the primal";
   return nullptr;
@@ -527,6 +531,7 @@ struct AdamWProgram {
     const c10::cuda::CUDAGuard guard(dev);
     wb::AdamArgs a{};
     if (lr_dev) {
+      if (const char* why = unfit(*lr_dev)) bad(std::string("AdamW.step: lr") + why);
       if (lr_dev->numel() != 1 || lr_dev->device() != dev || (lr_dev->scalar_type() != at::kFloat && lr_dev->scalar_type() != at::kDouble))
         bad("AdamW.step: lr is a number, or a float32 or float64 tensor of one element on the parameters' device");
       a.lr_ptr = lr_dev->const_data_ptr();
