@@ -66,3 +66,29 @@ def test_tensors_of_transforms_are_refused():
                 transform(call)(x[0] if transform is torch.func.grad else x)
     with pytest.raises(ValueError, match="wrapper"):
         grad_norm([torch._efficientzerotensor((4,))])
+
+
+@gpu
+@pytest.mark.parametrize("states", ["fp32", "fp8"])
+def test_captured_step_follows_rebound_parameters(states):
+    params, grads, opt = _setup(states=states, seed=5, master=True)
+    twin, _, ref = _setup(states=states, seed=5, master=True)
+    for o in (opt, ref):
+        o.step(grads, max_norm=1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = opt.step(grads, max_norm=1.0)
+    first = {n: p.clone() for n, p in params.items()}
+    moved = {n: p.clone() for n, p in params.items()}
+    opt.rebind(moved)
+    junk = [torch.full((1 << 12,), 255, dtype=torch.uint8, device="cuda") for _ in range(64)]      # takes what was given back
+    for k in range(3):
+        for i, g in enumerate(grads.values()):
+            g.copy_(_rand(tuple(g.shape), g.dtype, 10 * k + i, 0.1))
+        graph.replay()
+        assert torch.equal(norm, ref.step(grads, max_norm=1.0))
+    torch.cuda.synchronize()
+    assert len(junk) == 64 and opt.step_count == ref.step_count == 4
+    assert all(torch.equal(p, twin[n]) for n, p in moved.items())
+    assert all(torch.equal(p, first[n]) for n, p in params.items())          # the old memory is left alone

@@ -400,6 +400,7 @@ struct AdamWProgram {
     return host.to(dev);
   }
 
+  // The parameters' rows, into one table for the optimizer's life: captured steps hold its address.
   void upload_tensors() {
     std::vector<wb::AdamTensor> t;
     ptrs.clear();
@@ -407,7 +408,12 @@ struct AdamWProgram {
       ptrs.push_back(reinterpret_cast<uint64_t>(params[i].const_data_ptr()));
       t.push_back({ptrs[i], (uint64_t)params[i].numel(), offsets[i], float_code(params[i].scalar_type()), decay[i]});
     }
-    tables = upload(t.data(), t.size() * sizeof(wb::AdamTensor));
+    const c10::cuda::CUDAGuard guard(dev);
+    const size_t bytes = t.size() * sizeof(wb::AdamTensor);
+    if (!tables.defined()) tables = at::empty({(int64_t)bytes}, f32_options().dtype(at::kByte));
+    check(cudaMemcpyAsync(tables.mutable_data_ptr(), t.data(), bytes, cudaMemcpyHostToDevice, c10::cuda::getCurrentCUDAStream()),
+          "AdamW set-up");
+    settle();
   }
 
   // A tensor's slice of a flat state buffer, in the order of the parameter's memory.
@@ -457,7 +463,6 @@ struct AdamWProgram {
     const c10::cuda::CUDAGuard guard(dev);
     check(cudaDeviceSynchronize(), "AdamW.rebind");       // steps in flight on any stream read the old table
     upload_tensors();
-    settle();
   }
 
   // Collects the gradients of this step, and what the norm reads of them.

@@ -133,7 +133,9 @@ class AdamW:
 
     def rebind(self, params: Mapping[str, torch.Tensor]) -> None:
         """Go on with the same parameters at new addresses (their memory was released and
-        allocated again, e.g. by an engine that shares the GPU)."""
+        allocated again, e.g. by an engine that shares the GPU).  Waits for the GPU.  A captured
+        step follows: from now on its replays update the parameters where they are now, from
+        gradients where they were at the capture."""
         if list(params) != self.names:
             raise ValueError("AdamW.rebind: the parameters' names or their order differ")
         self._program.rebind(list(params.values()))
