@@ -92,3 +92,28 @@ def test_captured_step_follows_rebound_parameters(states):
     assert len(junk) == 64 and opt.step_count == ref.step_count == 4
     assert all(torch.equal(p, twin[n]) for n, p in moved.items())
     assert all(torch.equal(p, first[n]) for n, p in params.items())          # the old memory is left alone
+
+
+@gpu
+@pytest.mark.parametrize("states", ["fp32", "fp8"])
+def test_optimizer_released_while_its_step_waits(states):
+    """The step waits on a side stream behind other work; what the optimizer held is not given to anyone else before it ran."""
+    params, grads, opt = _setup([(1 << 20,)], torch.bfloat16, states=states, master=True)
+    twin, _, ref = _setup([(1 << 20,)], torch.bfloat16, states=states, master=True)
+    ref.step(grads, max_norm=1.0)
+    held = {t.data_ptr(): t.nbytes for t in opt.states().values()}
+    sizes = sorted(held.values())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    ran = torch.cuda.Event()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)                         # half a second
+        opt.step(grads, max_norm=1.0)
+        ran.record()
+    del opt
+    others = [torch.full((n,), 0x55, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(2)]
+    assert not ran.query()                                       # else this test shows nothing
+    for o in others:
+        assert not any(a < o.data_ptr() + o.nbytes and o.data_ptr() < a + n for a, n in held.items())
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, twin[n]) for n, p in params.items())

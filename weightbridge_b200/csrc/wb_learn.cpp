@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <limits>
@@ -310,6 +311,7 @@ struct AdamWProgram {
   std::vector<uint32_t> chunk_start;
   Tensor tables, chunks, clock, m, v, m_scale, v_scale, master;
   std::vector<uint64_t> grads;
+  std::vector<c10::cuda::CUDAStream> streams;      // that the allocator knows of
   int64_t total = 0;
   uint32_t chunk = wb::kAdamTile;
   double beta1, beta2, eps;
@@ -566,10 +568,21 @@ struct AdamWProgram {
     a.lr = lr;
     a.eps = eps;
     a.max_norm = max_norm;
-    check(wb::launch_adamw(a, grads.data(), chunk_start.data(), sms, c10::cuda::getCurrentCUDAStream()), "AdamW launch");
+    const auto stream = c10::cuda::getCurrentCUDAStream();
+    used_on(stream);
+    check(wb::launch_adamw(a, grads.data(), chunk_start.data(), sms, stream), "AdamW launch");
     for (const Tensor& p : params)
       if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();       // autograd sees the change
     return norm.defined() ? py::cast(norm) : py::none();
+  }
+
+  // Steps may run on any stream.  The allocator is told of each stream once, so that an optimizer released
+  // behind its last step leaves its memory to others only when that step has run.
+  void used_on(const c10::cuda::CUDAStream& stream) {
+    if (std::find(streams.begin(), streams.end(), stream) != streams.end()) return;
+    for (const Tensor& t : {tables, chunks, clock, m, v, m_scale, v_scale, master})
+      if (t.defined()) t.record_stream(stream.unwrap());
+    streams.push_back(stream);
   }
 
   at::TensorOptions f32_options() const { return params[0].options().dtype(at::kFloat).requires_grad(false); }

@@ -48,7 +48,8 @@ class AdamW:
 
     The states are flat buffers (``states()``); every tensor's slice starts at a multiple of 128
     elements, in the order of ``params``.  The step count lives on the device, so a captured step
-    can be replayed; a step runs on the current stream of the parameters' device.  fp32 arithmetic
+    can be replayed (while the optimizer lives); a step runs on the current stream of the parameters'
+    device.  fp32 arithmetic
     with the hardware's approximate root and reciprocal (relative errors of 2^-23).
     """
 
