@@ -117,3 +117,17 @@ def test_optimizer_released_while_its_step_waits(states):
         assert not any(a < o.data_ptr() + o.nbytes and o.data_ptr() < a + n for a, n in held.items())
     torch.cuda.synchronize()
     assert all(torch.equal(p, twin[n]) for n, p in params.items())
+
+
+@gpu
+def test_only_updated_parameters_change_their_version():
+    """A graph that saved a frozen parameter is still good after a step."""
+    p, q = (torch.nn.Parameter(_rand((40,), torch.float32, s)) for s in (1, 2))
+    e = torch.nn.Parameter(torch.empty(0, device="cuda"))
+    opt = AdamW({"p": p, "q": q, "e": e}, lr=0.1)
+    kept = (q * q).sum()
+    versions = q._version, p._version
+    opt.step({"p": torch.ones_like(p), "q": None, "e": torch.empty(0, device="cuda")}, max_norm=1.0)
+    assert q._version == versions[0] and p._version > versions[1]
+    kept.backward()
+    assert torch.equal(q.grad, 2 * q.detach())

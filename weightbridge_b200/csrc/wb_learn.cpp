@@ -571,8 +571,8 @@ struct AdamWProgram {
     const auto stream = c10::cuda::getCurrentCUDAStream();
     used_on(stream);
     check(wb::launch_adamw(a, grads.data(), chunk_start.data(), sms, stream), "AdamW launch");
-    for (const Tensor& p : params)
-      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();       // autograd sees the change
+    for (size_t i = 0; i < params.size(); ++i)          // autograd sees the change of those that took part
+      if (grads[i] && !params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
     return norm.defined() ? py::cast(norm) : py::none();
   }
 
