@@ -10,6 +10,7 @@ import torch
 from ._ext import ext
 
 STATE_BLOCK = 128           # elements that share a scale in the 8-bit states
+MAX_BETA2_FP8 = 0.95        # the longest memory that 8-bit second moments keep up with
 
 
 def grad_norm(tensors: Mapping[str, torch.Tensor] | Iterable[torch.Tensor], group: Any = None) -> torch.Tensor:
@@ -40,8 +41,12 @@ class AdamW:
     order of dimensions).  They are updated in place.  Of an FSDP trainer's DTensors, their local
     tensors (``parallel.fsdp.convert_to_wb`` returns those) with the gradients' local tensors.  ``states``: ``"fp32"``, or ``"fp8"``:
     both moments as e4m3 with one fp32 scale per 128 elements, 2.06 bytes a parameter instead of
-    8 (the second moment as its root).  An 8-bit second moment follows changes of a few percent a
-    step only through its block's largest element: use a ``beta2`` of at most 0.99 with it.
+    8 (the second moment as its root).  Codes are rounded to nearest, 3 to 6 % from their neighbours'
+    borders, and a root decays by ``sqrt(beta2)`` a step: it follows because its block's scale moves, and
+    only up to ``beta2`` = 0.95 (normal gradients: 5 % too large in the median there, 17 % at 0.97, 40 % and
+    more from 0.98 on, and elements whose gradients become small stop), so larger ones are refused.  A
+    block whose largest root stands still to a few percent keeps its other roots from decaying.
+    ``betas``: (0.9, 0.999), with 8-bit states (0.9, 0.95).
     ``master``: keep fp32 master weights of 16-bit parameters (taken from the parameters now);
     without them an update below half a step of the 16-bit type is lost.  ``no_decay``: names
     without weight decay, or a function of the name.
@@ -53,13 +58,18 @@ class AdamW:
     with the hardware's approximate root and reciprocal (relative errors of 2^-23).
     """
 
-    def __init__(self, params: Mapping[str, torch.Tensor], lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
+    def __init__(self, params: Mapping[str, torch.Tensor], lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] | None = None,
                  eps: float = 1e-8, weight_decay: float = 0.01, *, states: str = "fp32", master: bool = False,
                  no_decay: Iterable[str] | Callable[[str], bool] = ()):
         if states not in ("fp32", "fp8"):
             raise ValueError(f"AdamW: states must be 'fp32' or 'fp8', not {states!r}")
+        if betas is None:
+            betas = (0.9, MAX_BETA2_FP8 if states == "fp8" else 0.999)
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"AdamW: betas must be in [0, 1), not {betas}")
+        if states == "fp8" and betas[1] > MAX_BETA2_FP8:
+            raise ValueError(f"AdamW: 8-bit second moments do not follow a beta2 above {MAX_BETA2_FP8} (given: {betas[1]}): "
+                             "use a smaller one, or states='fp32'")
         if not 2.0 ** -126 <= eps < float("inf") or not 0.0 <= weight_decay < float("inf"):
             raise ValueError("AdamW: eps must be a positive normal fp32 number and weight_decay not negative")
         self._check_lr(lr)
