@@ -167,3 +167,33 @@ def test_8_bit_second_moments_over_many_steps():
     for part in (ratio[::2], ratio[1::2]):
         assert abs(math.log(float(part.median()))) <= math.log(1 + 2.0 ** -4)
         assert 0.75 < float(part.quantile(0.01)) and float(part.quantile(0.99)) < 1.5
+
+
+def test_8_bit_first_moments_refuse_long_memories():
+    p = {"a": torch.ones(4)}
+    for beta1 in (0.981, 0.99, 0.999):
+        with pytest.raises(ValueError, match="beta1"):
+            AdamW(p, betas=(beta1, 0.95), states="fp8")
+        with pytest.raises(ValueError, match="CUDA"):            # not refused for its betas
+            AdamW(p, betas=(beta1, 0.95))
+    with pytest.raises(ValueError, match="CUDA"):
+        AdamW(p, betas=(0.98, 0.95), states="fp8")
+
+
+@gpu
+@pytest.mark.parametrize("beta1,most", [(0.9, 0.09), (0.98, 0.2)])
+def test_8_bit_first_moments_over_many_steps(beta1, most):
+    """Normal gradients with means of a third of their size: what the codes' rounding adds up to (an
+    emulation of the definition gives 0.059 and 0.134 of the moments)."""
+    n = 128 * 256
+    opt = AdamW({"p": torch.zeros(n, device="cuda")}, lr=1e-3, betas=(beta1, 0.95), weight_decay=0.0, states="fp8")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    mean = 0.3 * torch.randn(n, device="cuda", generator=g)
+    m = torch.zeros(n, dtype=torch.float64, device="cuda")
+    for _ in range(1000):
+        grad = torch.randn(n, device="cuda", generator=g) + mean
+        opt.step({"p": grad})
+        m = beta1 * m + (1 - beta1) * grad.double()
+    st = opt.states()
+    got = (st["exp_avg"].float().view(-1, 128) * st["exp_avg_scale"][:, None]).view(-1).double()
+    assert float((got - m).norm() / m.norm()) < most
