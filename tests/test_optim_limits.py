@@ -197,3 +197,19 @@ def test_8_bit_first_moments_over_many_steps(beta1, most):
     st = opt.states()
     got = (st["exp_avg"].float().view(-1, 128) * st["exp_avg_scale"][:, None]).view(-1).double()
     assert float((got - m).norm() / m.norm()) < most
+
+
+@gpu
+def test_moments_that_are_not_numbers_stay_visible_in_8_bits():
+    """The second moment of a NaN gradient is a NaN code, like the first; the block's others stay numbers."""
+    params = {"p": torch.ones(256, device="cuda")}
+    opt = AdamW(params, states="fp8")
+    g = torch.ones(256, device="cuda")
+    g[3] = math.nan
+    for _ in range(2):
+        opt.step({"p": g})
+        g[3] = 1.0
+        for key in ("exp_avg", "rms"):
+            bad = opt.states()[key].float().isnan()
+            assert bool(bad[3]) and int(bad.sum()) == 1
+    assert int(params["p"].isnan().sum()) == 1

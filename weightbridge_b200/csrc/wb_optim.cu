@@ -97,10 +97,10 @@ __device__ __forceinline__ float block_inverse(float amax) {
   return fminf(q, 8.507059173e37f);         // 2^126, also where the above is not a number (zero and tiny blocks)
 }
 
-// r in units of the scale; a positive r keeps at least the smallest code
+// r in units of the scale; a positive r keeps at least the smallest code, NaN stays
 __device__ __forceinline__ F2 root_codes(F2 r, float inv) {
   const F2 q = mul2(r, both(inv));
-  return {fmaxf(q.x, r.x > 0.f ? 0.001953125f : 0.f), fmaxf(q.y, r.y > 0.f ? 0.001953125f : 0.f)};
+  return {r.x > 0.f ? fmaxf(q.x, 0.001953125f) : q.x, r.y > 0.f ? fmaxf(q.y, 0.001953125f) : q.y};
 }
 
 // The states of E consecutive elements of one lane as they come from memory.
