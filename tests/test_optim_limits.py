@@ -213,3 +213,17 @@ def test_moments_that_are_not_numbers_stay_visible_in_8_bits():
             bad = opt.states()[key].float().isnan()
             assert bool(bad[3]) and int(bad.sum()) == 1
     assert int(params["p"].isnan().sum()) == 1
+
+
+@gpu
+@pytest.mark.parametrize("large", [2.0 ** 125, 2.0 ** 126, 1e38, 3.4e38])
+def test_moments_near_the_largest_number_in_8_bits(large):
+    """beta1 = 0: the first moment is the gradient; its block keeps it to half a step."""
+    g = torch.full((256,), large, device="cuda")
+    g[1] = -large / 2
+    g[128:] = 1.0
+    opt = AdamW({"p": torch.ones(256, device="cuda")}, betas=(0.0, 0.95), states="fp8")
+    opt.step({"p": g})
+    st = opt.states()
+    got = st["exp_avg"].float().view(-1, 128).double() * st["exp_avg_scale"][:, None].double()
+    assert bool(((got.view(-1) - g.double()).abs() <= g.double().abs() * 2.0 ** -4).all())

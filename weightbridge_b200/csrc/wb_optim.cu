@@ -80,8 +80,9 @@ __device__ __forceinline__ F2 decode2(uint32_t q) {
 
 __device__ __forceinline__ uint32_t encode2(F2 x) { return __nv_cvt_float2_to_fp8x2(make_float2(x.x, x.y), __NV_SATFINITE, __NV_E4M3); }
 
-// Scale of a block, amax / 448, and 448 / amax, each with one correction step after the product
-// (the reciprocal of the rounded scale would round once more).  A block of tiny values keeps a
+// Scale of a block, amax / 448, and 448 / amax, each a product with an approximate reciprocal and one
+// Newton step of the quotient: q + (a - b q) / b, whose residual a fused multiply-add leaves exact but for one
+// rounding (the reciprocal of the rounded scale would round once more).  A block of tiny values keeps a
 // normal scale, whose reciprocal is finite; a block of zeros has scale 1.
 __device__ __forceinline__ float block_scale(float amax) {
   constexpr float kInv = 1.f / kE4M3Max;
@@ -91,9 +92,9 @@ __device__ __forceinline__ float block_scale(float amax) {
   return amax > 0.f ? fmaxf(q, 1.17549435e-38f) : 1.f;
 }
 __device__ __forceinline__ float block_inverse(float amax) {
-  const float r = reciprocal(amax);
-  float q = kE4M3Max * r;
-  q = fmaf(fmaf(-amax, q, kE4M3Max), r, q);
+  const float r = reciprocal(0.25f * amax);  // 4 / amax: a normal number up to the largest amax
+  float q = 0.25f * kE4M3Max * r;
+  q = fmaf(fmaf(-amax, q, kE4M3Max), 0.25f * r, q);
   return fminf(q, 8.507059173e37f);         // 2^126, also where the above is not a number (zero and tiny blocks)
 }
 
