@@ -227,3 +227,26 @@ def test_moments_near_the_largest_number_in_8_bits(large):
     st = opt.states()
     got = st["exp_avg"].float().view(-1, 128).double() * st["exp_avg_scale"][:, None].double()
     assert bool(((got.view(-1) - g.double()).abs() <= g.double().abs() * 2.0 ** -4).all())
+
+
+def test_eps_below_what_32_bits_can_hold_is_refused():
+    p = {"a": torch.ones(4)}
+    for eps in (0.0, 1e-40, 1e-30, 1e-20, 2.0 ** -51):
+        with pytest.raises(ValueError, match="eps"):
+            AdamW(p, eps=eps)
+    with pytest.raises(ValueError, match="CUDA"):
+        AdamW(p, eps=2.0 ** -50)
+
+
+@gpu
+@pytest.mark.parametrize("states", ["fp32", "fp8"])
+def test_small_gradients_take_small_steps(states):
+    """Gradients down to 1e-40 at the smallest eps: a first step of g / (|g| + eps).  A second moment below
+    2^-126 may count as 0: with beta2 = 0.95 that leaves out a root of at most 2^-63 / sqrt(0.05) < 2^-60.8
+    beside eps, so 2^-10.8 of a step that is itself below 2^-10.8."""
+    eps = 2.0 ** -50
+    g = torch.logspace(-40, 0, 41, device="cuda", dtype=torch.float64).repeat_interleave(128)
+    params = {"p": torch.zeros(g.numel(), device="cuda")}
+    AdamW(params, lr=1.0, betas=(0.9, 0.95), weight_decay=0.0, eps=eps, states=states).step({"p": g.float()})
+    want = -g / (g + eps)
+    assert float((params["p"].double() - want).abs().max()) <= 2.0 ** -20

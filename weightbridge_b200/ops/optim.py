@@ -10,6 +10,9 @@ import torch
 from ._ext import ext
 
 STATE_BLOCK = 128           # elements that share a scale in the 8-bit states
+# Squares below 2^-126 are no normal fp32 numbers: roots below 2^-63 may count as 0, and eps alone must keep the step
+# on such gradients small.  From 2^-50 on an update is off by at most 1.5e-5 of lr (beta2 = 0.999; 3e-7 at 0.95).
+MIN_EPS = 2.0 ** -50
 MAX_BETA1_FP8, MAX_BETA2_FP8 = 0.98, 0.95       # the longest memories that 8-bit moments keep up with
 
 
@@ -48,7 +51,7 @@ class AdamW:
     block whose largest root stands still to a few percent keeps its other roots from decaying.  The
     first moment's rounding adds up to 6 % of it at ``beta1`` = 0.9, 13 % at 0.98 and 18 to 36 % at 0.99:
     above 0.98 it is refused, too.
-    ``betas``: (0.9, 0.999), with 8-bit states (0.9, 0.95).
+    ``betas``: (0.9, 0.999), with 8-bit states (0.9, 0.95).  ``eps``: at least 2^-50 (9e-16).
     ``master``: keep fp32 master weights of 16-bit parameters (taken from the parameters now);
     without them an update below half a step of the 16-bit type is lost.  ``no_decay``: names
     without weight decay, or a function of the name.
@@ -73,8 +76,8 @@ class AdamW:
             if states == "fp8" and betas[k] > most:
                 raise ValueError(f"AdamW: 8-bit moments do not follow a beta{k + 1} above {most} (given: {betas[k]}): "
                                  "use a smaller one, or states='fp32'")
-        if not 2.0 ** -126 <= eps < float("inf") or not 0.0 <= weight_decay < float("inf"):
-            raise ValueError("AdamW: eps must be a positive normal fp32 number and weight_decay not negative")
+        if not MIN_EPS <= eps < float("inf") or not 0.0 <= weight_decay < float("inf"):
+            raise ValueError("AdamW: eps must be finite and at least 2^-50 (9e-16), and weight_decay finite and not negative")
         self._check_lr(lr)
         self.lr = lr
         self.betas, self.eps, self.weight_decay = tuple(map(float, betas)), float(eps), float(weight_decay)
