@@ -250,3 +250,23 @@ def test_small_gradients_take_small_steps(states):
     AdamW(params, lr=1.0, betas=(0.9, 0.95), weight_decay=0.0, eps=eps, states=states).step({"p": g.float()})
     want = -g / (g + eps)
     assert float((params["p"].double() - want).abs().max()) <= 2.0 ** -20
+
+
+@gpu
+@pytest.mark.parametrize("states", ["fp32", "fp8"])
+def test_master_weights_reread_from_the_parameters(states):
+    params, grads, opt = _setup(states=states, seed=9, master=True)
+    opt.step(grads)
+    for i, p in enumerate(params.values()):
+        p.copy_(_rand(tuple(p.shape), p.dtype, 300 + i, 0.5))    # loaded from a checkpoint, say
+    opt.read_master()
+    for n, w in opt.slices(opt.states()["master"]).items():
+        assert torch.equal(w, params[n].float())
+    _step_and_check(params, grads, opt)
+    moved = {n: (2 * p).clone() for n, p in params.items()}
+    opt.rebind(moved)
+    opt.read_master()
+    _step_and_check(moved, grads, opt, max_norm=1.0)
+    plain = _setup(states=states, seed=9)[2]
+    with pytest.raises(ValueError, match="no master weights"):
+        plain.read_master()

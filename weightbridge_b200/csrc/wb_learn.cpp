@@ -423,7 +423,10 @@ struct AdamWProgram {
     return at::as_strided(flat, params[i].sizes(), params[i].strides(), (int64_t)offsets[i]);
   }
 
+  // The master weights from the parameters' present values.
   void read_master() {
+    if (!master.defined()) bad("AdamW.read_master: there are no master weights");
+    const c10::cuda::CUDAGuard guard(dev);
     at::NoGradGuard no_grad;
     for (size_t i = 0; i < params.size(); ++i) slice(master, i).copy_(params[i].detach());
   }
@@ -606,7 +609,12 @@ void bind_learn(py::module_& m) {
       .def("step", &AdamWProgram::step)
       .def("grad_sum_sq", &AdamWProgram::grad_sum_sq)
       .def("rebind", &AdamWProgram::rebind)
-      .def("read_master", &AdamWProgram::read_master)
+      .def("read_master", [](AdamWProgram& p) {
+        const c10::cuda::CUDAGuard guard(p.dev);
+        check(cudaDeviceSynchronize(), "AdamW.read_master");     // steps in flight on any stream
+        p.read_master();
+        p.settle();
+      })
       .def("slice", [](const AdamWProgram& p, const Tensor& flat, size_t i) { return p.slice(flat, i); })
       .def_property("step_count", &AdamWProgram::get_step, &AdamWProgram::set_step)
       .def_readonly("total", &AdamWProgram::total)

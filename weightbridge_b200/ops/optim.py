@@ -52,7 +52,8 @@ class AdamW:
     first moment's rounding adds up to 6 % of it at ``beta1`` = 0.9, 13 % at 0.98 and 18 to 36 % at 0.99:
     above 0.98 it is refused, too.
     ``betas``: (0.9, 0.999), with 8-bit states (0.9, 0.95).  ``eps``: at least 2^-50 (9e-16).
-    ``master``: keep fp32 master weights of 16-bit parameters (taken from the parameters now);
+    ``master``: keep fp32 master weights of 16-bit parameters (taken from the parameters now, and by
+    ``read_master``: values written into the parameters otherwise do not last);
     without them an update below half a step of the 16-bit type is lost.  ``no_decay``: names
     without weight decay, or a function of the name.
 
@@ -156,6 +157,13 @@ class AdamW:
         if list(params) != self.names:
             raise ValueError("AdamW.rebind: the parameters' names or their order differ")
         self._program.rebind(list(params.values()))
+
+    def read_master(self) -> None:
+        """Take the fp32 master weights from the parameters' present values, as the constructor did.
+        A step goes on from the master weights and overwrites the parameters, so whoever changes those
+        (a checkpoint loaded into them, weights restored before or after ``rebind``) calls this next.
+        Waits for the GPU."""
+        self._program.read_master()
 
     def state_dict(self) -> dict:
         """The step count, the names and the state buffers (not copies)."""
