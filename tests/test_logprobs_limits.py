@@ -115,3 +115,107 @@ def test_tensors_of_transforms_are_refused():
             transform(lambda y: token_logprobs(y, t if y.dim() == 2 else t[0]).logprobs.sum())(x)
         with pytest.raises(ValueError, match="wrapper"):
             transform(lambda y: token_logprobs(x, y).logprobs.sum())(t.float() if transform is torch.func.grad else t)
+
+
+def _warp_a_row(rows, vocab, dtype):
+    """Whether the rows are many and short enough for a warp each (the rule of the launch)."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n = 1024 // dtype.itemsize
+    tiles = (vocab + n - 1) // n + 1
+    return tiles <= 65 and tiles * sms * 2 <= rows * 3
+
+
+def _mixed(rows, vocab, dtype, seed, pad=0, start=0):
+    """Rows of every kind, as a view of rows that are `pad` columns longer; (logits, tokens, rows without NaN)."""
+    x, t = _inputs(rows, vocab + pad, dtype, seed=seed, vocab=vocab)
+    x = x[:, start:start + vocab]
+    at = torch.arange(rows, device="cuda") % 23
+    low = torch.finfo(dtype).min
+    x[at == 3] = -math.inf                                       # empty
+    half = torch.arange(vocab, device="cuda") % 2 == 0
+    x[(at == 5)[:, None] & half] = -math.inf
+    x[(at == 7)[:, None] & half] = low
+    x[at == 9] = low
+    x[at == 11, -1] = 60.0
+    x[at == 13, 0] = math.nan
+    x[at == 15, vocab // 2] = math.inf
+    t[at == 17] = vocab                                          # no such token
+    t[at == 19] = -1
+    t[at == 21] = -100
+    return x, t, (at != 13) & (at != 15) & (at != 17) & (at != 19)
+
+
+def _check_mixed(x, t, good, temperature=1.0):
+    vocab = x.shape[1]
+    leaf = x.detach().requires_grad_()
+    out = token_logprobs(leaf, t, temperature=temperature)
+    live = t != -100
+    bad = ~good & live
+    assert bool(out.logprobs[bad].isnan().all()) and not bool(out.logprobs[~bad].isnan().any())
+    g = torch.Generator(device="cuda").manual_seed(2)
+    g1, g2 = (torch.randn(t.shape, device="cuda", generator=g) for _ in range(2))
+    d, = torch.autograd.grad((out.logprobs, out.entropy), leaf, (g1, g2))
+    assert bool(d[bad & ~torch.isneginf(x).all(1)].isnan().all())
+    keep_rows = good | ~live
+    xs, ts = x[keep_rows], t[keep_rows]
+    lp, h, logp, keep, z, p = _oracle(xs, ts, vocab, temperature)
+    tol_lp, tol_h = _bounds(z, p, lp, vocab)
+    _close(out.logprobs[keep_rows], lp, tol_lp, "logprobs")
+    _close(out.entropy[keep_rows], h, tol_h, "entropy")
+    _check_grad(d[keep_rows], g1[keep_rows], g2[keep_rows], lp, h, logp, p, keep, ts, vocab, temperature, tol_lp, tol_h)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,pad,start", [(10000, 1, 0, 0), (9990, 33, 0, 0), (5001, 1000, 0, 0), (2400, 1501, 7, 3), (10007, 2049, 1, 1), (4096, 9001, 0, 0),
+                                                  (4097, 4096, 8, 5)])
+def test_a_warp_a_row(dtype, rows, vocab, pad, start):
+    """More rows than the grid has warps, aligned and not, with ignored, masked, empty and NaN rows between the others."""
+    assert _warp_a_row(rows, vocab, dtype)
+    x, t, good = _mixed(rows, vocab, dtype, seed=rows, pad=pad, start=start)
+    _check_mixed(x, t, good, temperature=0.8)
+    t[0] = t[-1] = -100
+    t[rows // 4:rows // 4 + min(4736, rows // 2)] = -100         # as many in a row as a B200's grid has warps
+    _check_mixed(x, t, good)
+    t[:] = -100
+    leaf = x.detach().requires_grad_()
+    out = token_logprobs(leaf, t)
+    d, = torch.autograd.grad(out.logprobs.sum() + out.entropy.sum(), leaf)
+    assert not bool(out.logprobs.any()) and not bool(out.entropy.any()) and not bool(d.any())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tiles", [2, 9, 64, 65, 66])
+def test_row_counts_around_the_warp_rule(dtype, tiles):
+    vocab = (tiles - 1) * (1024 // dtype.itemsize)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    border = (tiles * sms * 2 + 2) // 3
+    assert _warp_a_row(border, vocab, dtype) == (tiles <= 65) and not _warp_a_row(border - 1, vocab, dtype)
+    for rows in (border - 1, border):
+        x, t, good = _mixed(rows, vocab, dtype, seed=rows)
+        _check_mixed(x, t, good)
+
+
+@gpu
+@pytest.mark.parametrize("rows,vocab", [(149, 131072 - 256), (149, 131073), (150, 140001), (2, 2 ** 21), (1, 2 ** 21 - 5), (300, 152000)])
+@pytest.mark.parametrize("top_k", [1, 20, 32])
+def test_alternatives_of_wide_rows(rows, vocab, top_k):
+    """More tiles a CTA than two a thread: their maxima are selected by search instead of by counting."""
+    x, t = _inputs(rows, vocab, torch.float32, seed=16)
+    x[0] = x[0].round()                                          # many ties
+    if rows > 8:
+        x[1] = 0.25                                              # one value: the lowest ids
+        x[2] = -math.inf
+        x[3] = -math.inf
+        x[3, vocab - 7] = 1.0                                    # one column, then ties of -inf
+        x[4] = torch.arange(vocab, device="cuda").float()
+        x[5] = -x[4]
+        x[6] = -0.0
+        x[6, ::3] = 0.0
+        x[7] = x[7].bfloat16().float()
+        t[2] = -100
+    for part in (slice(0, 12), slice(rows - 1, rows)):           # the oracle sorts in 64 bits
+        want = _check(x[part], t[part], top_k=top_k, grad=False)
+        out = token_logprobs(x, t, top_k=top_k)
+        assert torch.equal(out.top_ids[part], want.top_ids)

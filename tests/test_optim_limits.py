@@ -270,3 +270,40 @@ def test_master_weights_reread_from_the_parameters(states):
     plain = _setup(states=states, seed=9)[2]
     with pytest.raises(ValueError, match="no master weights"):
         plain.read_master()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,gdtype,master,elements", [
+    (torch.bfloat16, None, False, 160_000_000), (torch.bfloat16, None, True, 160_000_000), (torch.bfloat16, torch.float32, True, 80_000_000),
+    (torch.float32, None, False, 80_000_000)])
+def test_8_bit_steps_whose_copies_run_ahead(dtype, gdtype, master, elements):
+    """Enough elements for work items of several tiles, so that every warp fills its shared memory again
+    and again, and every CTA takes several items; blocks of different size, ends of every kind."""
+    sizes = [(elements // 2 + 12345,), (3, elements // 8 + 77), (elements // 16,), (5000,), (129,)]
+    params, grads, opt = _setup(sizes, dtype, gdtype, seed=30, states="fp8", master=master)
+    for k in range(2):
+        for i, g in enumerate(grads.values()):
+            flat = g.view(-1)
+            g.copy_(_rand(tuple(g.shape), g.dtype, 500 + 10 * k + i, 1e-2))
+            flat *= (1 + torch.arange(flat.numel(), device="cuda") // 128 % (37 + k)).to(flat.dtype)
+        _step_and_check(params, grads, opt, max_norm=1.0 if k else None)
+
+
+@gpu
+@pytest.mark.parametrize("shift", [0, 3])
+@pytest.mark.parametrize("dtype,gdtype,master", [(torch.bfloat16, torch.float32, True), (torch.float32, None, False)])
+def test_fp32_steps_of_several_items_a_block(dtype, gdtype, master, shift):
+    params, grads, opt = _setup([(15_000_001,), (64,), (6_000_000,)], dtype, gdtype, shift=shift, seed=31, master=master)
+    for k in range(2):
+        _step_and_check(params, grads, opt, max_norm=1.0 if k else None)
+        for i, g in enumerate(grads.values()):
+            g.copy_(_rand(tuple(g.shape), g.dtype, 600 + i, 1e-3))
+
+
+@gpu
+def test_8_bit_steps_at_odd_addresses_of_several_items_a_block():
+    params, grads, opt = _setup([(40_000_001,), (700_001,)], torch.bfloat16, shift=3, seed=32, states="fp8", master=True)
+    for k in range(2):
+        _step_and_check(params, grads, opt, max_norm=1.0 if k else None)
+        for i, g in enumerate(grads.values()):
+            g.copy_(_rand(tuple(g.shape), g.dtype, 700 + i, 1e-3))
