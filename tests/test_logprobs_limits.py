@@ -219,3 +219,19 @@ def test_alternatives_of_wide_rows(rows, vocab, top_k):
         want = _check(x[part], t[part], top_k=top_k, grad=False)
         out = token_logprobs(x, t, top_k=top_k)
         assert torch.equal(out.top_ids[part], want.top_ids)
+
+
+@gpu
+def test_next_tokens_by_ignoring_the_last_position():
+    """The whole logits with the last position ignored: what the shifted views give, to the bit."""
+    full, _ = _inputs(4 * 65, 5003, torch.bfloat16, seed=17)
+    full = full.view(4, 65, 5003).requires_grad_()
+    ids = torch.randint(0, 5003, (4, 65), device="cuda")
+    g = torch.randn(4, 65, device="cuda")
+    view = token_logprobs(full[:, :-1], ids[:, 1:])
+    whole = token_logprobs(full, torch.nn.functional.pad(ids[:, 1:], (0, 1), value=-100))
+    for a, b in zip(view[:2], whole[:2]):
+        assert torch.equal(a, b[:, :-1]) and not bool(b[:, -1].any())
+    d, = torch.autograd.grad(view[:2], full, (g[:, :-1], g[:, :-1]))
+    e, = torch.autograd.grad(whole[:2], full, (g, g))
+    assert torch.equal(d, e)

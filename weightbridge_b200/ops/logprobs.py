@@ -33,6 +33,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, vocab: int | N
     (vocabulary padding) take no part and get a zero gradient.  ``top_k``: 0 to 32 alternatives
     ordered by logit, ties by the lower id (of at most 2^21 columns); they carry no gradient.
 
+    For the tokens one position on, ``logits[:, :-1]`` does for scoring; where a gradient is taken give
+    the whole logits and ``ignore_index`` as the last position's token: torch's backward of the
+    slice would zero and fill a whole gradient behind the kernel, more than it moves itself.
+
     Rows whose token is ``ignore_index`` are not read: log probability and entropy 0, gradient
     0, alternatives -1 at -inf.  Columns of -inf have probability 0; a row that has no other is
     empty: log probability -inf, entropy 0, gradient 0.  NaN or +inf in a row, or a token
