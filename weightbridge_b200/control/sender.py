@@ -1063,7 +1063,8 @@ class WeightSender:
         with its sampled ``tokens`` against this trainer's, from ``logits`` computed with the weights
         of the last sync (``policy_gap`` has the arguments; with padded positions, tokens of
         ``ignore_index``).  ``version``: the weights version the rollout sampled with; ``ValueError``
-        where the last completed sync carried another.  ``tolerance``: ``TransferError`` where the
+        where the last completed sync carried another (a sync of some ``names`` carries its version, too: the
+        names it left out are taken to be unchanged).  ``tolerance``: ``TransferError`` where the
         mean difference is above it.  This rank's tokens only; no other rank takes part."""
         if version is not None and version != self.version:
             raise ValueError(f"the rollout sampled with weights version {version}, the last sync carried {self.version}")

@@ -24,7 +24,8 @@ def grad_norm(tensors: Mapping[str, torch.Tensor] | Iterable[torch.Tensor], grou
     its local tensor).  The sum
     runs in a fixed order: the same inputs give the same bits.  ``group``: a process group over
     which the squares are summed; a tensor that several of its ranks hold counts once per rank.
-    Squares are formed in 32 bits: a gradient above 1.8e19 makes the norm infinite.
+    Squares are formed, and up to 64 of them added, in 32 bits, all else in 64: gradients above 2.3e18 can
+    make the norm infinite, those below 1.1e-19 lose bits of their squares, and below 2.6e-23 they do not count.
     """
     if not isinstance(tensors, (dict, list, tuple)):
         tensors = dict(tensors) if isinstance(tensors, Mapping) else list(tensors)
@@ -99,6 +100,8 @@ class AdamW:
              max_norm: float | None = None, group: Any = None) -> torch.Tensor | None:
         """One update from ``grads`` (name -> tensor of the parameter's type or fp32; default: the
         parameters' ``.grad``).  A parameter without a gradient is left alone in this step.
+        The bias correction counts this optimizer's steps, not a parameter's own: one whose first
+        gradient comes late takes a smaller first step than lr (betas 0.9 and 0.95: 0.45 of it).
 
         ``lr``: this step's learning rate (default: ``self.lr``); a one-element tensor on the
         device is read there, so that it can change under a captured step.  ``max_norm``: scale
