@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -52,16 +53,19 @@ std::string shape_of(const Tensor& t) {
 // Why a tensor's memory may not be read as its values, or null.  Wrappers of other tensors (DTensor, what
 // torch.func hands to a function) and lazy zeros have no memory of their own, some an address of 0; a
 // forward mode derivative would be lost without a word.
-const char* unfit(const Tensor& t) {
+const char* unfit(const Tensor& t, bool dual) {
   using c10::DispatchKey;
   constexpr c10::DispatchKeySet kWrappers({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
                                            DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched, DispatchKey::ZeroTensor});
   if (t.layout() != at::kStrided || t.key_set().has_any(kWrappers))
     return " is a sparse tensor or a wrapper (DTensor, a transform's): give the plain local tensor (to_local())";
   if (t.is_neg()) return " is negated lazily, its memory holds other values: give resolve_neg() of it";
-  if (t._fw_grad(0).defined()) return " carries a derivative of forward mode, which is not implemented: give the primal";
+  if (dual && t._fw_grad(0).defined()) return " carries a derivative of forward mode, which is not implemented: give the primal";
   return nullptr;
 }
+
+// Whether forward mode derivatives can be about: asked once a call, since asking a view for its own takes 25 ns.
+bool duals() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 
 int sm_count(int device) {
   static std::array<int, 64> known{};          // one attribute query per device; the value never changes
@@ -220,7 +224,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, const std::optional<int64_t>& columns, double temperature,
                          int64_t top_k, int64_t ignore_index) {
   for (const Tensor* x : {&logits, &tokens})
-    if (const char* why = unfit(*x)) bad(std::string("token_logprobs: an argument") + why);
+    if (const char* why = unfit(*x, duals())) bad(std::string("token_logprobs: an argument") + why);
   if (logits.dim() < 1) bad("token_logprobs: logits need a vocabulary dimension");
   const int64_t cols = logits.size(-1), vocab = columns.value_or(cols);
   if (!float_code(logits.scalar_type())) bad("token_logprobs: logits must be bfloat16, float16 or float32");
@@ -269,12 +273,13 @@ wb::NormTensor norm_tensor(const Tensor& x) {
 py::tuple sum_squares(const py::object& tensors) {
   std::vector<wb::NormTensor> t;
   const Tensor* first = nullptr;
+  const bool dual = duals();
   auto add = [&](PyObject* o) {
     if (o == Py_None) return;
     if (!THPVariable_Check(o)) throw py::type_error("grad_norm: not a tensor");
     const Tensor& x = THPVariable_Unpack(o);
     if (!first) first = &x;
-    if (const char* why = unfit(x)) bad(std::string("grad_norm: a tensor") + why);
+    if (const char* why = unfit(x, dual)) bad(std::string("grad_norm: a tensor") + why);
     if (!x.is_cuda() || x.device() != first->device()) bad("grad_norm: all tensors must be CUDA tensors of one device");
     if (!float_code(x.scalar_type())) bad("grad_norm: tensors must be bfloat16, float16 or float32");
     if (!dense(x)) bad("grad_norm: a tensor of shape " + shape_of(x) + " has holes or overlaps in memory");
@@ -379,7 +384,7 @@ struct AdamWProgram {
   }
 
   void check_param(const Tensor& p, const std::string& name) const {
-    if (const char* why = unfit(p)) bad("AdamW: " + name + why);
+    if (const char* why = unfit(p, duals())) bad("AdamW: " + name + why);
     if (!p.is_cuda() || p.device() != dev) bad("AdamW: " + name + " is not on the CUDA device of the first parameter");
     if (!float_code(p.scalar_type())) bad("AdamW: " + name + " must be bfloat16, float16 or float32");
     if (!dense(p)) bad("AdamW: " + name + " has holes or overlaps in memory; give the whole parameter, not a view of part of it");
@@ -474,7 +479,7 @@ struct AdamWProgram {
   void collect(const py::object& src, std::vector<wb::NormTensor>* normed) {
     grads.assign(params.size(), 0);
     Py_ssize_t found = 0;
-    const bool dict = !src.is_none();
+    const bool dict = !src.is_none(), dual = duals();
     if (dict && !PyDict_Check(src.ptr())) throw py::type_error("AdamW.step: gradients are a dict of name -> tensor, or None for the parameters' .grad");
     for (size_t i = 0; i < params.size(); ++i) {
       const Tensor& p = params[i];
@@ -495,7 +500,7 @@ struct AdamWProgram {
         g = &p.grad();
       }
       if (!g || !g->defined()) continue;
-      if (const char* why = unfit(*g)) bad("AdamW.step: the gradient of " + names[i] + why);
+      if (const char* why = unfit(*g, dual)) bad("AdamW.step: the gradient of " + names[i] + why);
       if (!g->is_cuda() || g->device() != dev) bad("AdamW.step: the gradient of " + names[i] + " is on another device");
       if (g->sizes() != p.sizes()) bad("AdamW.step: the gradient of " + names[i] + " has shape " + shape_of(*g) + ", not " + shape_of(p));
       if (g->scalar_type() != p.scalar_type() && g->scalar_type() != at::kFloat)
@@ -541,7 +546,7 @@ struct AdamWProgram {
     const c10::cuda::CUDAGuard guard(dev);
     wb::AdamArgs a{};
     if (lr_dev) {
-      if (const char* why = unfit(*lr_dev)) bad(std::string("AdamW.step: lr") + why);
+      if (const char* why = unfit(*lr_dev, duals())) bad(std::string("AdamW.step: lr") + why);
       if (lr_dev->numel() != 1 || lr_dev->device() != dev || (lr_dev->scalar_type() != at::kFloat && lr_dev->scalar_type() != at::kDouble))
         bad("AdamW.step: lr is a number, or a float32 or float64 tensor of one element on the parameters' device");
       a.lr_ptr = lr_dev->const_data_ptr();
