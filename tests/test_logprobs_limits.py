@@ -235,3 +235,17 @@ def test_next_tokens_by_ignoring_the_last_position():
     d, = torch.autograd.grad(view[:2], full, (g[:, :-1], g[:, :-1]))
     e, = torch.autograd.grad(whole[:2], full, (g, g))
     assert torch.equal(d, e)
+
+
+def test_released_storage_is_refused():
+    """A tensor whose storage was given back, whole (its address is 0) or in part, still has its sizes."""
+    x, t = torch.randn(4, 10), torch.zeros(4, dtype=torch.long)
+    for left in (0, 31):
+        gone, no_tokens = torch.randn(4, 10), torch.zeros(4, dtype=torch.long)
+        for y in (gone, no_tokens):
+            y.untyped_storage().resize_(left)
+        for logits, tokens in ((gone, t), (x, no_tokens)):
+            with pytest.raises(ValueError, match="storage"):
+                token_logprobs(logits, tokens)
+    with pytest.raises(ValueError, match="CUDA"):                # nothing to read: not refused for that
+        token_logprobs(torch.randn(0, 10), torch.zeros(0, dtype=torch.long))

@@ -307,3 +307,25 @@ def test_8_bit_steps_at_odd_addresses_of_several_items_a_block():
         _step_and_check(params, grads, opt, max_norm=1.0 if k else None)
         for i, g in enumerate(grads.values()):
             g.copy_(_rand(tuple(g.shape), g.dtype, 700 + i, 1e-3))
+
+
+def test_released_storage_is_refused():
+    """A tensor whose storage was given back, whole (its address is 0) or in part, still has its sizes."""
+    for left in (0, 15):
+        x = torch.ones(4)
+        x.untyped_storage().resize_(left)
+        for call in (lambda: AdamW({"a": x}), lambda: grad_norm([x])):
+            with pytest.raises(ValueError, match="storage"):
+                call()
+
+
+@gpu
+def test_released_gradient_is_refused():
+    p = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    opt = AdamW({"a": p})
+    for dtype in (torch.bfloat16, torch.float32):
+        g = torch.ones(64, dtype=dtype, device="cuda")
+        g.untyped_storage().resize_(0)
+        with pytest.raises(ValueError, match="storage"):
+            opt.step({"a": g})
+    assert opt.step_count == 0 and bool((p == 1).all())

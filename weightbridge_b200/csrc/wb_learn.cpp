@@ -4,6 +4,7 @@
 // fit raises ValueError.  Outputs and scratch come from torch's allocator on the current stream of
 // the tensors' device, and the kernels run on that stream, so calls on different streams share nothing.
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
@@ -57,8 +58,13 @@ const char* unfit(const Tensor& t, bool dual) {
   using c10::DispatchKey;
   constexpr c10::DispatchKeySet kWrappers({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
                                            DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched, DispatchKey::ZeroTensor});
-  if (t.layout() != at::kStrided || t.key_set().has_any(kWrappers))
+  if (t.key_set().has_any(kWrappers) || t.layout() != at::kStrided)
     return " is a sparse tensor or a wrapper (DTensor, a transform's): give the plain local tensor (to_local())";
+  if (const int64_t n = t.numel()) {
+    size_t bytes = (size_t)(t.storage_offset() + n) * t.itemsize();
+    if (!t.is_non_overlapping_and_dense()) bytes = at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.itemsize(), t.storage_offset());
+    if (bytes > t.storage().nbytes()) return " has less memory than its shape asks for: its storage was released";
+  }
   if (t.is_neg()) return " is negated lazily, its memory holds other values: give resolve_neg() of it";
   if (dual && t._fw_grad(0).defined()) return " carries a derivative of forward mode, which is not implemented: give the primal";
   return nullptr;
