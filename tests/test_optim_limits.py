@@ -329,3 +329,19 @@ def test_released_gradient_is_refused():
         with pytest.raises(ValueError, match="storage"):
             opt.step({"a": g})
     assert opt.step_count == 0 and bool((p == 1).all())
+
+
+@gpu
+def test_parameters_of_another_size_or_type_at_the_same_address():
+    """`p.data` may be set to a part of itself: the address stays, the table's size is another."""
+    for change in (lambda x: x[:5], lambda x: x.view(torch.bfloat16)):
+        p = torch.nn.Parameter(torch.ones(64, device="cuda"))
+        opt = AdamW({"a": p})
+        address = p.data_ptr()
+        p.data = change(p.data)
+        assert p.data_ptr() == address
+        with pytest.raises(RuntimeError, match="rebind"):
+            opt.step({"a": torch.ones_like(p)})
+        with pytest.raises(ValueError, match="another shape"):
+            opt.rebind({"a": p})
+        assert opt.step_count == 0

@@ -318,6 +318,8 @@ struct AdamWProgram {
   std::vector<std::string> names;
   std::vector<Tensor> params;
   std::vector<uint64_t> ptrs, offsets;
+  struct Shape { int64_t numel; at::ScalarType type; std::vector<int64_t> sizes, strides; };
+  std::vector<Shape> shapes;       // as they were given: a parameter's `data` may be set to another tensor
   std::vector<float> decay;
   std::vector<uint32_t> chunk_start;
   Tensor tables, chunks, clock, m, v, m_scale, v_scale, master;
@@ -340,6 +342,7 @@ struct AdamWProgram {
     for (size_t i = 0; i < params.size(); ++i) {
       check_param(params[i], names[i]);
       narrow |= params[i].scalar_type() != at::kFloat;
+      shapes.push_back({params[i].numel(), params[i].scalar_type(), params[i].sizes().vec(), params[i].strides().vec()});
       offsets.push_back((uint64_t)total);
       decay.push_back((float)decay_[i]);
       total += (params[i].numel() + wb::kStateBlock - 1) / wb::kStateBlock * wb::kStateBlock;
@@ -431,7 +434,7 @@ struct AdamWProgram {
 
   // A tensor's slice of a flat state buffer, in the order of the parameter's memory.
   Tensor slice(const Tensor& flat, size_t i) const {
-    return at::as_strided(flat, params[i].sizes(), params[i].strides(), (int64_t)offsets[i]);
+    return at::as_strided(flat, shapes[i].sizes, shapes[i].strides, (int64_t)offsets[i]);
   }
 
   // The master weights from the parameters' present values.
@@ -465,7 +468,7 @@ struct AdamWProgram {
     if (p.size() != params.size()) bad("AdamW.rebind: another number of parameters");
     for (size_t i = 0; i < p.size(); ++i) {
       check_param(p[i], names[i]);
-      if (p[i].sizes() != params[i].sizes() || p[i].strides() != params[i].strides() || p[i].scalar_type() != params[i].scalar_type())
+      if (p[i].sizes() != at::IntArrayRef(shapes[i].sizes) || p[i].strides() != at::IntArrayRef(shapes[i].strides) || p[i].scalar_type() != shapes[i].type)
         bad("AdamW.rebind: " + names[i] + " has another shape, stride or type");
     }
     auto before = params;
@@ -491,6 +494,8 @@ struct AdamWProgram {
       const Tensor& p = params[i];
       if (reinterpret_cast<uint64_t>(p.const_data_ptr()) != ptrs[i])
         throw std::runtime_error("AdamW.step: " + names[i] + " moved in memory; call rebind()");
+      if (p.numel() != shapes[i].numel || p.scalar_type() != shapes[i].type || !dense(p))
+        throw std::runtime_error("AdamW.step: " + names[i] + " has another size or type than at the constructor; call rebind() with what it was");
       const Tensor* g = nullptr;
       if (dict) {
         PyObject* o = PyDict_GetItemWithError(src.ptr(), py_names[i].ptr());
