@@ -249,3 +249,30 @@ def test_released_storage_is_refused():
                 token_logprobs(logits, tokens)
     with pytest.raises(ValueError, match="CUDA"):                # nothing to read: not refused for that
         token_logprobs(torch.randn(0, 10), torch.zeros(0, dtype=torch.long))
+
+
+@gpu
+def test_saved_tensors_that_hooks_replace():
+    """What a hook gives back is checked again: kept on the host and returned packed it is fine, left there it is refused."""
+    full, _ = _inputs(8, 703, torch.float32, seed=18)
+    ids = torch.randint(0, 700, (8,), device="cuda")
+    leaf = full[:, 3:].detach().requires_grad_()
+    g = torch.randn(8, device="cuda")
+
+    def grad():
+        out = token_logprobs(leaf, ids)
+        return torch.autograd.grad((out.logprobs, out.entropy), leaf, (g, g))[0]
+
+    want = grad()
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.allclose(grad(), want, rtol=1e-6, atol=0)   # rows at other alignments
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x.cpu(), lambda x: x):
+        with pytest.raises(RuntimeError, match="hook"):
+            grad()
+    for change in (lambda x: x[:4] if x.dim() else x, lambda x: x.double() if x.is_floating_point() else x):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, change):
+            with pytest.raises(RuntimeError, match="hook"):
+                grad()
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x.t().contiguous().t() if x.dim() == 2 else x):
+        assert torch.allclose(grad(), want, rtol=1e-6, atol=0)   # the same values in another order of memory
+    assert torch.equal(grad(), want)

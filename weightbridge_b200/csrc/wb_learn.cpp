@@ -187,12 +187,18 @@ Tensor row_grad(const Tensor& g, const float*& ptr, int64_t& stride) {
   return t;
 }
 
+[[noreturn]] void replaced() {
+  throw std::runtime_error("token_logprobs: a hook brought a saved tensor back on another device or in another shape or type");
+}
+
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
                                                 int64_t vocab, double temperature, int64_t top_k, int64_t ignore_index) {
     const LogprobOptions o{vocab, ignore_index, temperature, top_k};
     LogprobResult r = run_logprobs(logits, tokens, o, true);
     ctx->save_for_backward({logits, tokens, r.stats, r.entropy});
+    ctx->saved_data["rows"] = tokens.numel();
+    ctx->saved_data["cols"] = logits.size(-1);
     ctx->saved_data["vocab"] = vocab;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -206,7 +212,18 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     if (at::GradMode::is_enabled())
       throw std::runtime_error("token_logprobs: the gradient has no second derivative (create_graph=True)");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2], &entropy = saved[3];
+    // Hooks on saved tensors may have brought other ones back.
+    const Tensor &tokens = saved[1], stats = saved[2].contiguous(), entropy = saved[3].contiguous();
+    const Tensor logits = saved[0].size(-1) > 1 && saved[0].stride(-1) != 1 ? saved[0].contiguous() : saved[0];
+    for (const Tensor* x : {&logits, &tokens, &stats, &entropy})
+      if (unfit(*x, false) || !x->is_cuda() || x->device() != logits.device()) replaced();
+    for (const Tensor& g : grads)
+      if (g.defined() && g.device() != logits.device()) replaced();
+    if (!float_code(logits.scalar_type()) || logits.dim() != tokens.dim() + 1 || tokens.sizes() != logits.sizes().slice(0, tokens.dim()) ||
+        logits.size(-1) != ctx->saved_data["cols"].toInt() || (tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) ||
+        tokens.numel() != ctx->saved_data["rows"].toInt() || stats.scalar_type() != at::kFloat || entropy.scalar_type() != at::kFloat ||
+        stats.numel() != 2 * tokens.numel() || entropy.numel() != tokens.numel())
+      replaced();
     const LogprobOptions o{ctx->saved_data["vocab"].toInt(), ctx->saved_data["ignore_index"].toInt(),
                            ctx->saved_data["temperature"].toDouble(), 0};
     const c10::cuda::CUDAGuard guard(logits.device());
