@@ -366,10 +366,10 @@ struct AdamWProgram {
     }
     const c10::cuda::CUDAGuard guard(dev);
     sms = sm_count(dev.index());
-    // A work item: one tile with fp32 states (436M parameters: 2099 us with one, 2120 with eight; 1.45M: 7.7
-    // and 12.4).  8-bit states overlap their loads within an item: eight tiles, as long as every SM
-    // gets 32 items (604M parameters: 1340 us with one, 1085 with eight, 1101 with sixteen; 24M:
-    // 105 with one, 117 with eight).
+    // A work item: one tile with fp32 states (a clipped step over 1.45M parameters: 14.5 us with one, 19.1 with
+    // eight; over 436M 2417 and 2375, on another GPU the other way).  8-bit states overlap their loads within
+    // an item: eight tiles, as long as every SM gets 32 items (604M parameters: 1620 us with one, 1280 with
+    // eight; 24M at odd addresses: 95 with one, 112 with eight).
     chunk = fp8 ? 8 * wb::kAdamTile : wb::kAdamTile;
     while (chunk > wb::kAdamTile && total < (int64_t)sms * 32 * chunk) chunk /= 2;
     for (const Tensor& p : params) {
