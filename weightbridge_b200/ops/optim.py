@@ -43,8 +43,8 @@ class AdamW:
     ``params``: name -> tensor, e.g. ``dict(model.named_parameters())`` or the tensors a layout
     allocates; bf16, fp16 or fp32 on one CUDA device, each filling its memory without holes (any
     order of dimensions).  They are updated in place.  Of an FSDP trainer's DTensors, their local
-    tensors (``parallel.fsdp.convert_to_wb`` returns those) with the gradients' local tensors.  ``states``: ``"fp32"``, or ``"fp8"``:
-    both moments as e4m3 with one fp32 scale per 128 elements, 2.06 bytes a parameter instead of
+    tensors (``parallel.fsdp.convert_to_wb`` returns those) with the gradients' local tensors.
+    ``states``: ``"fp32"``, or ``"fp8"``: both moments as e4m3 with one fp32 scale per 128 elements, 2.06 bytes a parameter instead of
     8 (the second moment as its root).  Codes are rounded to nearest, 3 to 6 % from their neighbours'
     borders, and a root decays by ``sqrt(beta2)`` a step: it follows because its block's scale moves, and
     only up to ``beta2`` = 0.95 (normal gradients: 5 % too large in the median there, 17 % at 0.97, 40 % and
@@ -61,8 +61,9 @@ class AdamW:
     The states are flat buffers (``states()``); every tensor's slice starts at a multiple of 128
     elements, in the order of ``params``.  The step count lives on the device, so a captured step
     can be replayed (while the optimizer lives); a step runs on the current stream of the parameters'
-    device.  fp32 arithmetic
-    with the hardware's approximate root and reciprocal (relative errors of 2^-23).
+    device.  Steps of one optimizer follow one another: whoever takes them on several streams orders
+    those, and ``step_count``, ``state_dict`` and ``load_state_dict`` behind them.  fp32 arithmetic with the hardware's
+    approximate root and reciprocal (relative errors of 2^-23).
     """
 
     def __init__(self, params: Mapping[str, torch.Tensor], lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] | None = None,
